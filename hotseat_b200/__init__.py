@@ -27,6 +27,8 @@ LIB_PATH = os.path.join(_HERE, "libhotseat.so")
 HS_OK = 0
 HS_E_ARG, HS_E_IO, HS_E_CUDA, HS_E_STATE, HS_E_NOMEM, HS_E_UNSUPPORTED = -1, -2, -3, -4, -5, -6
 TOKEN_MAJOR, HEAD_MAJOR = 0, 1
+F32, F16, BF16 = 0, 1, 2
+POS_NONE = 0xFFFFFFFF
 NUMERIC_REFERENCE, NUMERIC_FAST, NUMERIC_TC = 0, 1, 2
 DONE_REASONS = {0: "", 1: "eos", 2: "max_tokens", 3: "context full"}
 
@@ -145,6 +147,23 @@ _SIGS = {
     "hs_kv_write_runs": (C.c_int, [_P, _P, C.c_uint64, _P, C.c_uint64]),
     "hs_kv_live_ranges_between": (C.c_uint64, [C.POINTER(KvSpec), C.c_uint32, C.c_uint32, _P, C.c_uint64]),
     "hs_runs_to_byte_runs": (C.c_uint64, [_P, C.c_uint64, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64]),
+    "hs_kv8_alloc": (C.c_int, [C.c_int, C.POINTER(KvSpec), C.c_uint32, C.c_uint32, C.c_uint64, C.POINTER(_P)]),
+    "hs_kv8_alloc_model": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(_P)]),
+    "hs_kv8_open_ipc": (C.c_int, [_P, C.c_char_p, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(_P)]),
+    "hs_kv8_block": (C.c_int, [_P, C.POINTER(C.c_uint32)]),
+    "hs_kv8_live_ranges_between": (C.c_uint64, [C.POINTER(KvSpec), C.c_uint32, C.c_uint32, C.c_uint32, _P,
+                                                C.c_uint64]),
+    "hs_kv8_set_new": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.POINTER(_P)]),
+    "hs_kv8_set_free": (None, [_P]),
+    "hs_kv8_set_check": (C.c_int, [_P, _P]),
+    "hs_kv8_append": (C.c_int, [_P, C.c_uint32, C.c_uint32, _P, _P, _P, _P, C.c_uint32, C.c_uint64, C.c_uint64, _P]),
+    "hs_kv8_read": (C.c_int, [_P, C.c_uint32, C.c_uint32, _P, _P, _P, _P, C.c_uint32, C.c_uint64, C.c_uint64, _P]),
+    "hs_kv8_attend": (C.c_int, [_P, C.c_uint32, C.c_uint32, _P, _P, _P, C.c_uint64, C.c_uint64, _P, C.c_uint64,
+                                C.c_uint64, C.c_uint32, C.c_float, _P]),
+    "hs_logprobs": (C.c_int, [C.c_int, _P, C.c_uint32, C.c_uint64, C.c_uint32, C.c_uint32, _P, C.c_uint32, _P, _P,
+                              _P, _P, _P, _P]),
+    "hs_scratch_logprobs": (C.c_int, [_P, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P]),
+    "hs_batch_logprobs": (C.c_int, [_P, _P, C.c_uint32, C.c_uint32, _P, _P, _P, _P, _P]),
     "hs_scratch_new": (C.c_int, [_P, C.POINTER(_P)]),
     "hs_scratch_free": (None, [_P]),
     "hs_forward": (C.c_int, [_P, _P, C.c_uint32, C.c_uint32, _P]),
@@ -266,6 +285,12 @@ class Model:
     def kv(self, layout=TOKEN_MAJOR, page_size=4096):
         return Kv.alloc(self, layout, page_size)
 
+    def kv8(self, layout=TOKEN_MAJOR, block=1, page_size=4096):
+        """An 8-bit KV region of this model's shape (hs_kv8_alloc_model)."""
+        h = C.c_void_p()
+        _check(_lib.hs_kv8_alloc_model(self._h, layout, block, page_size, C.byref(h)))
+        return Kv(h, self)
+
     def scratch(self):
         return Scratch(self)
 
@@ -285,12 +310,23 @@ class Kv:
         _check(_lib.hs_kv_info(handle, C.byref(self.spec), C.byref(b), C.byref(ps), C.byref(npg)))
         self.bytes, self.page_size, self.n_pages = b.value, ps.value, npg.value
         self.n_words = (self.n_pages + 63) // 64
+        blk = C.c_uint32()
+        _check(_lib.hs_kv8_block(handle, C.byref(blk)))
+        self.block = blk.value  # positions under one scale; 0: f32 rows
 
     @classmethod
     def alloc(cls, model, layout=TOKEN_MAJOR, page_size=4096):
         h = C.c_void_p()
         _check(_lib.hs_kv_alloc(model._h, layout, page_size, C.byref(h)))
         return cls(h, model)
+
+    @classmethod
+    def alloc8(cls, spec, block=1, page_size=4096, device=0, fingerprint=0):
+        """An 8-bit region of a given shape: int8 codes with one f32 scale per
+        `block` positions and KV head, K and V apart (hs_kv8_alloc)."""
+        h = C.c_void_p()
+        _check(_lib.hs_kv8_alloc(device, C.byref(spec), block, page_size, fingerprint, C.byref(h)))
+        return cls(h, None)
 
     def ipc_handle(self):
         """The region's CUDA IPC handle (bytes) for another process's open_ipc."""
@@ -304,6 +340,13 @@ class Kv:
         hand-over destination."""
         h = C.c_void_p()
         _check(_lib.hs_kv_open_ipc(model._h, bytes(handle), layout, page_size, C.byref(h)))
+        return cls(h, model)
+
+    @classmethod
+    def open_ipc8(cls, model, handle, layout=TOKEN_MAJOR, block=1, page_size=4096):
+        """open_ipc of an 8-bit region."""
+        h = C.c_void_p()
+        _check(_lib.hs_kv8_open_ipc(model._h, bytes(handle), layout, block, page_size, C.byref(h)))
         return cls(h, model)
 
     def close(self):
@@ -427,6 +470,151 @@ def runs_to_byte_runs(words, n_pages, page_size, live):
     return [(int(out[2 * i]), int(out[2 * i + 1])) for i in range(n)]
 
 
+def live_ranges_between8(spec, block, a, b):
+    n = _lib.hs_kv8_live_ranges_between(C.byref(spec), block, a, b, None, 0)
+    out = np.zeros(2 * max(n, 1), dtype=np.uint64)
+    _lib.hs_kv8_live_ranges_between(C.byref(spec), block, a, b, _ptr(out), n)
+    return [(int(out[2 * i]), int(out[2 * i + 1])) for i in range(n)]
+
+
+# Device tensors of the calls below: torch tensors (or anything with their
+# methods). Torch itself is not imported here: element types are known by name,
+# each looked up once.
+_DTYPE_NAMES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+_INDEX_NAMES = ("torch.int32", "torch.uint32")
+_dtypes = {}
+
+
+def _dtype(t):
+    """HS_* of a tensor's elements; -1 for 32-bit integers, None for others."""
+    try:
+        return _dtypes[t.dtype]
+    except KeyError:
+        name = str(t.dtype)
+        _dtypes[t.dtype] = -1 if name in _INDEX_NAMES else _DTYPE_NAMES.get(name)
+        return _dtypes[t.dtype]
+
+
+def _matrix(t, device, shape, name, dtype=None):
+    """A [rows, heads, head_dim] (or [rows, vocab]) tensor: its element type and strides."""
+    if t.get_device() != device or device < 0:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    dt = _dtype(t)
+    if dt is None or dt < 0 or (dtype is not None and dt != dtype):
+        raise ValueError(f"{name} has type {t.dtype}")
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name}: the elements of a row must be consecutive")
+    return dt, st
+
+
+def _vector(t, device, n, name, dtype=-1):
+    """A consecutive vector of n 32-bit elements: its pointer (None: NULL)."""
+    if t is None:
+        return None
+    if t.get_device() != device or device < 0:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
+    if t.shape != (n,) or _dtype(t) != dtype or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be a consecutive {'int32' if dtype < 0 else 'float32'} vector of {n}")
+    return t.data_ptr()
+
+
+class Kv8Set:
+    """8-bit KV regions as the slots of batched calls (hs_kv8_set). Row
+    matrices are device tensors [rows, heads, head_dim] (f32, f16 or bf16, any
+    row and head strides); pos [n] and row_start [n + 1] are int32 device
+    tensors: slot i's rows are row_start[i]..row_start[i + 1] - 1, at positions
+    pos[i], pos[i] + 1, ... (row_start None: one row for each slot). pos -1
+    marks a slot without rows. Calls enqueue on `stream` (a CUDA stream
+    handle; None: the default stream) and do not wait."""
+
+    def __init__(self, kvs, n_heads=0):
+        self.kvs = list(kvs)  # the regions must outlive the set
+        h = C.c_void_p()
+        _check(_lib.hs_kv8_set_new((C.c_void_p * len(self.kvs))(*[k._h.value for k in self.kvs]), len(self.kvs),
+                                   n_heads, C.byref(h)))
+        self._h = h
+        self.n, self.n_heads, self.spec = len(self.kvs), n_heads, self.kvs[0].spec
+        self._nkv, self._hd = self.spec.n_kv_heads, self.spec.head_dim
+        self._scale = self._hd ** -0.5
+
+    def close(self):
+        if getattr(self, "_h", None):
+            _lib.hs_kv8_set_free(self._h)
+            self._h = None
+
+    __del__ = close
+
+    def append(self, layer, k, v, pos, row_start=None, stream=None):
+        """Quantise rows of K and V [rows, n_kv_heads, head_dim] into `layer`."""
+        d = k.get_device()
+        shape = (k.shape[0], self._nkv, self._hd)
+        dt, st = _matrix(k, d, shape, "k")
+        if _matrix(v, d, shape, "v", dt)[1] != st:
+            raise ValueError("k and v must have the same strides")
+        _check(_lib.hs_kv8_append(self._h, layer, shape[0], _vector(row_start, d, self.n + 1, "row_start"),
+                                  _vector(pos, d, self.n, "pos"), k.data_ptr(), v.data_ptr(), dt, st[0], st[1],
+                                  stream))
+
+    def read(self, layer, k, v, pos, row_start=None, stream=None):
+        """The values of cached rows into k and v (either may be None)."""
+        t = k if k is not None else v
+        if t is None:
+            raise ValueError("k and v are both None")
+        d = t.get_device()
+        shape = (t.shape[0], self._nkv, self._hd)
+        dt, st = _matrix(t, d, shape, "k" if k is not None else "v")
+        if k is not None and v is not None and _matrix(v, d, shape, "v", dt)[1] != st:
+            raise ValueError("k and v must have the same strides")
+        _check(_lib.hs_kv8_read(self._h, layer, shape[0], _vector(row_start, d, self.n + 1, "row_start"),
+                                _vector(pos, d, self.n, "pos"), k.data_ptr() if k is not None else None,
+                                v.data_ptr() if v is not None else None, dt, st[0], st[1], stream))
+
+    def attend(self, layer, q, out, pos, row_start=None, scale=None, stream=None):
+        """Causal attention of rows q [rows, n_heads, head_dim] over the cached
+        positions up to each row's own, into out. scale None: head_dim ** -0.5."""
+        d = q.get_device()
+        shape = (q.shape[0], self.n_heads, self._hd)
+        dt, st = _matrix(q, d, shape, "q")
+        ot = _matrix(out, d, shape, "out", dt)[1]
+        _check(_lib.hs_kv8_attend(self._h, layer, shape[0], _vector(row_start, d, self.n + 1, "row_start"),
+                                  _vector(pos, d, self.n, "pos"), q.data_ptr(), st[0], st[1], out.data_ptr(), ot[0],
+                                  ot[1], dt, self._scale if scale is None else scale, stream))
+
+    def check(self, stream=None):
+        """Wait for `stream`; raises if a call since the last check met a row past max_ctx."""
+        _check(_lib.hs_kv8_set_check(self._h, stream))
+
+
+def logprobs(logits, ids=None, logp=None, entropy=None, rank=None, top_ids=None, top_logp=None, stream=None):
+    """Scores of logit rows (device tensor [rows, vocab], f32, f16 or bf16) into
+    the outputs given (device tensors): log probability and rank of the tokens
+    ids [rows] (int32), entropy, and the first `top` tokens of each row with
+    their log probabilities (top_ids int32 and top_logp [rows, top])."""
+    rows, vocab = logits.shape
+    d = logits.get_device()
+    dt, st = _matrix(logits, d, (rows, vocab), "logits")
+    top = 0
+    for t, name, want in ((top_ids, "top_ids", -1), (top_logp, "top_logp", F32)):
+        if t is None:
+            continue
+        n = t.shape[1]
+        if t.get_device() != d or t.shape[0] != rows or (top and n != top) or _dtype(t) != want or not t.is_contiguous():
+            raise ValueError(f"{name} must be a consecutive [rows, top] tensor of {'int32' if want < 0 else 'float32'}")
+        top = n
+    _check(_lib.hs_logprobs(d, logits.data_ptr(), dt, st[0], rows, vocab, _vector(ids, d, rows, "ids"), top,
+                            _vector(logp, d, rows, "logp", F32), _vector(entropy, d, rows, "entropy", F32),
+                            _vector(rank, d, rows, "rank"), top_ids.data_ptr() if top and top_ids is not None else None,
+                            top_logp.data_ptr() if top and top_logp is not None else None, stream))
+
+
+def _host_scores(rows, top):
+    return dict(logp=np.zeros(rows, np.float32), entropy=np.zeros(rows, np.float32), rank=np.zeros(rows, np.uint32),
+                top_ids=np.zeros((rows, top), np.uint32), top_logp=np.zeros((rows, top), np.float32))
+
+
 class Scratch:
     """Per-decode-thread device state: activations, logits, stream, graphs."""
 
@@ -457,6 +645,14 @@ class Scratch:
         out = C.c_double()
         _check(_lib.hs_scratch_nll(self._h, next_token, C.byref(out)))
         return out.value
+
+    def logprobs(self, next_token, top=0):
+        """Scores of the current logits: logp and rank of next_token, entropy,
+        top_ids and top_logp (host arrays, hs_scratch_logprobs)."""
+        o = _host_scores(1, top)
+        _check(_lib.hs_scratch_logprobs(self._h, next_token, top, _ptr(o["logp"]), _ptr(o["entropy"]), _ptr(o["rank"]),
+                                        _ptr(o["top_ids"]) if top else None, _ptr(o["top_logp"]) if top else None))
+        return {k: a[0] for k, a in o.items()}
 
     @property
     def stream(self):
@@ -555,6 +751,15 @@ class Batch:
         out = np.zeros(max(1, t.size), dtype=np.float64)
         _check(_lib.hs_batch_nll(self._h, _ptr(t), t.size, _ptr(out)))
         return out[: t.size]
+
+    def logprobs(self, next_tokens, top=0):
+        """Scores of the last forward's logits, slot by slot (hs_batch_logprobs)."""
+        t = np.ascontiguousarray(next_tokens, dtype=np.uint32)
+        o = _host_scores(t.size, top)
+        _check(_lib.hs_batch_logprobs(self._h, _ptr(t), t.size, top, _ptr(o["logp"]), _ptr(o["entropy"]),
+                                      _ptr(o["rank"]), _ptr(o["top_ids"]) if top else None,
+                                      _ptr(o["top_logp"]) if top else None))
+        return o
 
     @property
     def stream(self):

@@ -13,6 +13,10 @@ namespace hs {
 void set_error(const std::string& msg);
 int fail(int code, const std::string& msg);
 
+// Live byte ranges of positions [from, to) of a region in either format, as
+// hs_kv_live_ranges_between gives them.
+uint64_t kv_live_ranges(const hs_kv* kv, uint32_t from, uint32_t to, uint64_t* out, uint64_t cap);
+
 inline uint32_t f2u(float f) { uint32_t u; std::memcpy(&u, &f, 4); return u; }
 inline float u2f(uint32_t u) { float f; std::memcpy(&f, &u, 4); return f; }
 

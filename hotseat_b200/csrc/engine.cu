@@ -14,6 +14,8 @@
 #include "common.h"
 #include "gguf.h"
 #include "kernels.h"
+#include "kv8.h"
+#include "kv_region.h"
 
 namespace hs {
 
@@ -243,44 +245,6 @@ struct hs_model {
     }
 };
 
-struct hs_kv {
-    hs_kv_spec spec{};
-    int device = 0;
-    uint64_t bytes = 0, n_pages = 0, n_words = 0;
-    uint32_t page_size = 0, page_shift = 0;
-    float* base = nullptr;
-    uint64_t* dirty = nullptr;
-    uint64_t* harvest_buf = nullptr;
-    uint32_t* tracking = nullptr;
-    uint64_t fingerprint = 0;
-    cudaStream_t st = nullptr;
-    int n_sm = 148;
-    // byte-run transfers: packed staging (grown on demand), the run table
-    // (pinned upload buffer and device copy) and the event after its last use
-    uint8_t* stage = nullptr;
-    uint64_t stage_cap = 0;
-    hs::XferRun *tab_h = nullptr, *tab_dev = nullptr;
-    uint64_t tab_cap = 0;
-    cudaEvent_t tab_ev = nullptr;
-    bool ipc_view = false;  // `base` maps another process's region (hs_kv_open_ipc)
-    ~hs_kv() {
-        cudaSetDevice(device);
-        if (tab_ev) cudaEventSynchronize(tab_ev);
-        if (st) cudaStreamDestroy(st);
-        if (tab_ev) cudaEventDestroy(tab_ev);
-        cudaFreeHost(tab_h);
-        cudaFree(tab_dev);
-        cudaFree(stage);
-        if (ipc_view)
-            cudaIpcCloseMemHandle(base);
-        else
-            cudaFree(base);
-        cudaFree(dirty);
-        cudaFree(harvest_buf);
-        cudaFree(tracking);
-    }
-};
-
 struct hs_scratch {
     const hs_model* m = nullptr;
     cudaStream_t st = nullptr;
@@ -297,6 +261,7 @@ struct hs_scratch {
     float* wps = nullptr;
     double* nll = nullptr;          // perplexity score of the last forward (hs_scratch_nll)
     uint32_t* nll_next = nullptr;
+    uint32_t* scores = nullptr;     // hs_scratch_logprobs: the token and its scores
     cudaGraphExec_t g_fwd = nullptr, g_step = nullptr;
     const hs_kv* graph_kv = nullptr;
     uint32_t graph_kmax = 0;
@@ -326,7 +291,8 @@ struct hs_scratch {
         cudaFreeHost(trace_init);
         for (void* p : {(void*)x, (void*)qkv, (void*)att, (void*)hb, (void*)logits, (void*)tokens, (void*)cand,
                         (void*)argbuf, (void*)sc_global, (void*)att_part, (void*)att_cnt, (void*)kv_tab,
-                        (void*)tok_mem, (void*)sort_cand, (void*)wkeys, (void*)wps, (void*)nll, (void*)nll_next})
+                        (void*)tok_mem, (void*)sort_cand, (void*)wkeys, (void*)wps, (void*)nll, (void*)nll_next,
+                        (void*)scores})
             cudaFree(p);
     }
 };
@@ -429,6 +395,8 @@ int check_kv(const hs_model* m, const hs_kv* kv) {
     if (kv->spec.n_layers != c.n_layers || kv->spec.n_kv_heads != c.n_kv_heads || kv->spec.head_dim != c.head_dim ||
         kv->spec.max_ctx != c.max_ctx)
         return fail(HS_E_ARG, "KV cache shape does not match the model");
+    if (kv->block8 && m->numeric != HS_NUMERIC_TC)
+        return fail(HS_E_UNSUPPORTED, "an 8-bit KV region decodes on the tensor-core path only");
     if (kv->device != m->device) return fail(HS_E_ARG, "KV cache lives on another device than the model");
     return HS_OK;
 }
@@ -876,6 +844,114 @@ int validate_cfg(hs_scratch* s, const hs_sampler_cfg* cfg, uint32_t* kmax) {
 }  // namespace
 }  // namespace hs
 
+namespace hs {
+
+hs_kv_spec model_kv_spec(const hs_model* m, uint32_t layout) {
+    return hs_kv_spec{m->cfg.n_layers, m->cfg.n_kv_heads, m->cfg.head_dim, m->cfg.max_ctx, layout};
+}
+
+int kv_create(int device, const hs_kv_spec& spec, uint32_t block8, uint32_t page_size, uint64_t fingerprint,
+              const void* handle, hs_kv** out) {
+    if (spec.layout > 1) return fail(HS_E_ARG, "unknown KV layout");
+    if (page_size < 256 || (page_size & (page_size - 1))) return fail(HS_E_ARG, "page_size must be a power of two >= 256");
+    uint64_t bytes = (uint64_t)spec.n_layers * 2 * spec.max_ctx * spec.n_kv_heads * spec.head_dim * 4;
+    if (block8) {
+        int rc = kv8_check_shape(spec, block8);
+        if (rc) return rc;
+        bytes = kv8_geo(spec, block8).bytes();
+    }
+    int n_dev = 0;
+    HS_CUDA_TRY(cudaGetDeviceCount(&n_dev));
+    if (device < 0 || device >= n_dev) return fail(HS_E_ARG, "no such device");
+    HS_CUDA_TRY(cudaSetDevice(device));
+    auto kv = std::make_unique<hs_kv>();
+    kv->device = device;
+    kv->spec = spec;
+    kv->block8 = block8;
+    kv->bytes = bytes;
+    kv->page_size = page_size;
+    kv->page_shift = (uint32_t)__builtin_ctz(page_size);
+    kv->n_pages = (kv->bytes + page_size - 1) / page_size;
+    kv->n_words = (kv->n_pages + 63) / 64;
+    kv->fingerprint = fingerprint;
+    if (handle) {
+        cudaIpcMemHandle_t h;
+        std::memcpy(&h, handle, sizeof h);
+        void* p = nullptr;
+        HS_CUDA_TRY(cudaIpcOpenMemHandle(&p, h, cudaIpcMemLazyEnablePeerAccess));
+        kv->base = static_cast<float*>(p);
+        kv->ipc_view = true;
+    }
+    HS_CUDA_TRY(cudaStreamCreateWithFlags(&kv->st, cudaStreamNonBlocking));
+    if (!handle) {
+        HS_CUDA_TRY(cudaMalloc(&kv->base, kv->bytes));
+        HS_CUDA_TRY(cudaMemset(kv->base, 0, kv->bytes));
+    }
+    // A view is written and read, never decoded into: its own page bits
+    // exist only so that every region has them.
+    HS_CUDA_TRY(cudaMalloc(&kv->dirty, kv->n_words * 8));
+    HS_CUDA_TRY(cudaMemset(kv->dirty, 0, kv->n_words * 8));
+    HS_CUDA_TRY(cudaMalloc(&kv->harvest_buf, kv->n_words * 8));
+    HS_CUDA_TRY(cudaMalloc(&kv->tracking, 4));
+    HS_CUDA_TRY(cudaMemset(kv->tracking, 0, 4));
+    HS_CUDA_TRY(cudaEventCreateWithFlags(&kv->tab_ev, cudaEventDisableTiming));
+    HS_CUDA_TRY(cudaDeviceGetAttribute(&kv->n_sm, cudaDevAttrMultiProcessorCount, device));
+    HS_CUDA_TRY(cudaStreamSynchronize(nullptr));  // the fills above, before any non-blocking stream writes
+    *out = kv.release();
+    return HS_OK;
+}
+
+uint64_t kv_live_ranges(const hs_kv* kv, uint32_t from, uint32_t to, uint64_t* out, uint64_t cap) {
+    return kv->block8 ? hs_kv8_live_ranges_between(&kv->spec, kv->block8, from, to, out, cap)
+                      : hs_kv_live_ranges_between(&kv->spec, from, to, out, cap);
+}
+
+}  // namespace hs
+
+namespace hs {
+namespace {
+
+// hs_logprobs of `rows` rows of f32 logits on `st`, from and to host memory,
+// through a device buffer of `cap` rows made at the first use:
+// ids | logp | entropy | rank | top ids | top logp.
+int scores_to_host(uint32_t** buf, uint32_t cap, const float* logits, uint32_t rows, uint32_t vocab,
+                   const uint32_t* next, uint32_t top, float* logp, float* entropy, uint32_t* rank, uint32_t* top_ids,
+                   float* top_logp, cudaStream_t st) {
+    int rc = check_logprobs(rows, vocab, next, top, logp, rank, top_ids, top_logp);
+    if (rc) return rc;
+    for (uint32_t i = 0; next && i < rows; i++)
+        if (next[i] >= vocab) return fail(HS_E_ARG, "token out of range");
+    if (!rows) return HS_OK;
+    if (!*buf) HS_CUDA_TRY(cudaMalloc(buf, (size_t)cap * (4 + 2 * kLogprobTop) * 4));
+    uint32_t *ids = *buf, *at = ids + cap;
+    auto part = [&](uint64_t per) {
+        uint32_t* p = at;
+        at += (uint64_t)cap * per;
+        return p;
+    };
+    uint32_t *d_logp = part(1), *d_ent = part(1), *d_rank = part(1), *d_ids = part(kLogprobTop),
+             *d_tlp = part(kLogprobTop);
+    if (next) HS_CUDA_TRY(cudaMemcpyAsync(ids, next, (size_t)rows * 4, cudaMemcpyHostToDevice, st));
+    LogprobArgs a{logits, vocab, HS_F32, rows, vocab, next ? ids : nullptr, top,
+                  reinterpret_cast<float*>(logp ? d_logp : nullptr), reinterpret_cast<float*>(entropy ? d_ent : nullptr),
+                  rank ? d_rank : nullptr, top_ids ? d_ids : nullptr, reinterpret_cast<float*>(top_logp ? d_tlp : nullptr)};
+    cudaError_t e = launch_logprobs(a, st);
+    if (e != cudaSuccess) return fail(HS_E_CUDA, std::string("logprobs launch: ") + cudaGetErrorString(e));
+    auto down = [&](void* host, const uint32_t* dev, uint64_t n) {
+        return host ? cudaMemcpyAsync(host, dev, n * 4, cudaMemcpyDeviceToHost, st) : cudaSuccess;
+    };
+    HS_CUDA_TRY(down(logp, d_logp, rows));
+    HS_CUDA_TRY(down(entropy, d_ent, rows));
+    HS_CUDA_TRY(down(rank, d_rank, rows));
+    HS_CUDA_TRY(down(top_ids, d_ids, (uint64_t)rows * top));
+    HS_CUDA_TRY(down(top_logp, d_tlp, (uint64_t)rows * top));
+    HS_CUDA_TRY(cudaStreamSynchronize(st));
+    return HS_OK;
+}
+
+}  // namespace
+}  // namespace hs
+
 extern "C" {
 
 const char* hs_last_error(void) { return g_err.c_str(); }
@@ -1158,29 +1234,25 @@ int hs_model_tensor(const hs_model* m, const char* name, void* host, uint64_t by
 
 int hs_kv_alloc(const hs_model* m, uint32_t layout, uint32_t page_size, hs_kv** out) {
     if (!m || !out) return fail(HS_E_ARG, "null argument");
-    if (layout > 1) return fail(HS_E_ARG, "unknown KV layout");
-    if (page_size < 256 || (page_size & (page_size - 1))) return fail(HS_E_ARG, "page_size must be a power of two >= 256");
-    HS_CUDA_TRY(cudaSetDevice(m->device));
-    auto kv = std::make_unique<hs_kv>();
-    kv->device = m->device;
-    kv->spec = hs_kv_spec{m->cfg.n_layers, m->cfg.n_kv_heads, m->cfg.head_dim, m->cfg.max_ctx, layout};
-    kv->bytes = (uint64_t)kv->spec.n_layers * 2 * kv->spec.max_ctx * kv->spec.n_kv_heads * kv->spec.head_dim * 4;
-    kv->page_size = page_size;
-    kv->page_shift = (uint32_t)__builtin_ctz(page_size);
-    kv->n_pages = (kv->bytes + page_size - 1) / page_size;
-    kv->n_words = (kv->n_pages + 63) / 64;
-    kv->fingerprint = m->cfg.fingerprint;
-    HS_CUDA_TRY(cudaStreamCreateWithFlags(&kv->st, cudaStreamNonBlocking));
-    HS_CUDA_TRY(cudaMalloc(&kv->base, kv->bytes));
-    HS_CUDA_TRY(cudaMemset(kv->base, 0, kv->bytes));
-    HS_CUDA_TRY(cudaMalloc(&kv->dirty, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMemset(kv->dirty, 0, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMalloc(&kv->harvest_buf, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMalloc(&kv->tracking, 4));
-    HS_CUDA_TRY(cudaMemset(kv->tracking, 0, 4));
-    HS_CUDA_TRY(cudaEventCreateWithFlags(&kv->tab_ev, cudaEventDisableTiming));
-    kv->n_sm = m->n_sm;
-    *out = kv.release();
+    return kv_create(m->device, model_kv_spec(m, layout), 0, page_size, m->cfg.fingerprint, nullptr, out);
+}
+
+int hs_kv8_alloc_model(const hs_model* m, uint32_t layout, uint32_t block, uint32_t page_size, hs_kv** out) {
+    if (!m || !out) return fail(HS_E_ARG, "null argument");
+    if (!block) return fail(HS_E_ARG, "an 8-bit region needs a scale block");
+    return kv_create(m->device, model_kv_spec(m, layout), block, page_size, m->cfg.fingerprint, nullptr, out);
+}
+
+int hs_kv8_alloc(int device, const hs_kv_spec* spec, uint32_t block, uint32_t page_size, uint64_t fingerprint,
+                 hs_kv** out) {
+    if (!spec || !out) return fail(HS_E_ARG, "null argument");
+    if (!block) return fail(HS_E_ARG, "an 8-bit region needs a scale block");
+    return kv_create(device, *spec, block, page_size, fingerprint, nullptr, out);
+}
+
+int hs_kv8_block(const hs_kv* kv, uint32_t* block) {
+    if (!kv || !block) return fail(HS_E_ARG, "null argument");
+    *block = kv->block8;
     return HS_OK;
 }
 
@@ -1197,36 +1269,14 @@ int hs_kv_ipc_handle(hs_kv* kv, void* out, uint64_t out_bytes) {
 
 int hs_kv_open_ipc(const hs_model* m, const void* handle, uint32_t layout, uint32_t page_size, hs_kv** out) {
     if (!m || !handle || !out) return fail(HS_E_ARG, "null argument");
-    if (layout > 1) return fail(HS_E_ARG, "unknown KV layout");
-    if (page_size < 256 || (page_size & (page_size - 1))) return fail(HS_E_ARG, "page_size must be a power of two >= 256");
-    HS_CUDA_TRY(cudaSetDevice(m->device));
-    auto kv = std::make_unique<hs_kv>();
-    kv->device = m->device;
-    kv->spec = hs_kv_spec{m->cfg.n_layers, m->cfg.n_kv_heads, m->cfg.head_dim, m->cfg.max_ctx, layout};
-    kv->bytes = (uint64_t)kv->spec.n_layers * 2 * kv->spec.max_ctx * kv->spec.n_kv_heads * kv->spec.head_dim * 4;
-    kv->page_size = page_size;
-    kv->page_shift = (uint32_t)__builtin_ctz(page_size);
-    kv->n_pages = (kv->bytes + page_size - 1) / page_size;
-    kv->n_words = (kv->n_pages + 63) / 64;
-    kv->fingerprint = m->cfg.fingerprint;
-    cudaIpcMemHandle_t h;
-    std::memcpy(&h, handle, sizeof h);
-    void* p = nullptr;
-    HS_CUDA_TRY(cudaIpcOpenMemHandle(&p, h, cudaIpcMemLazyEnablePeerAccess));
-    kv->base = static_cast<float*>(p);
-    kv->ipc_view = true;
-    HS_CUDA_TRY(cudaStreamCreateWithFlags(&kv->st, cudaStreamNonBlocking));
-    // the view is written and read, never decoded into: its own page bits
-    // exist only so that every region has them
-    HS_CUDA_TRY(cudaMalloc(&kv->dirty, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMemset(kv->dirty, 0, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMalloc(&kv->harvest_buf, kv->n_words * 8));
-    HS_CUDA_TRY(cudaMalloc(&kv->tracking, 4));
-    HS_CUDA_TRY(cudaMemset(kv->tracking, 0, 4));
-    HS_CUDA_TRY(cudaEventCreateWithFlags(&kv->tab_ev, cudaEventDisableTiming));
-    kv->n_sm = m->n_sm;
-    *out = kv.release();
-    return HS_OK;
+    return kv_create(m->device, model_kv_spec(m, layout), 0, page_size, m->cfg.fingerprint, handle, out);
+}
+
+int hs_kv8_open_ipc(const hs_model* m, const void* handle, uint32_t layout, uint32_t block, uint32_t page_size,
+                    hs_kv** out) {
+    if (!m || !handle || !out) return fail(HS_E_ARG, "null argument");
+    if (!block) return fail(HS_E_ARG, "an 8-bit region needs a scale block");
+    return kv_create(m->device, model_kv_spec(m, layout), block, page_size, m->cfg.fingerprint, handle, out);
 }
 
 int hs_kv_fingerprint(const hs_kv* kv, uint64_t* out) {
@@ -1292,9 +1342,9 @@ int hs_kv_hash(hs_kv* kv, uint32_t n_pos, uint64_t* out) {
     // kv.rs:267-274 with hash::Wide (hash.rs:63-126), over bytes staged to the host.
     if (!kv || !out) return fail(HS_E_ARG, "null argument");
     if (n_pos > kv->spec.max_ctx) return fail(HS_E_ARG, "n_pos past max_ctx");
-    const uint64_t nr = hs_kv_live_ranges_between(&kv->spec, 0, n_pos, nullptr, 0);
+    const uint64_t nr = kv_live_ranges(kv, 0, n_pos, nullptr, 0);
     std::vector<uint64_t> r(2 * nr);
-    hs_kv_live_ranges_between(&kv->spec, 0, n_pos, r.data(), nr);
+    kv_live_ranges(kv, 0, n_pos, r.data(), nr);
     uint64_t lanes[4] = {0x243f6a8885a308d3ull, 0x13198a2e03707344ull, 0xa4093822299f31d0ull, 0x082efa98ec4e6c89ull};
     uint64_t total = 0;
     const uint64_t P = 0x00000100000001b3ull;
@@ -1476,7 +1526,7 @@ int hs_kv_write_runs(hs_kv* kv, const uint64_t* runs, uint64_t n_runs, const voi
 
 int hs_kv_peer_copy(hs_kv* src, hs_kv* dst, const uint64_t* runs, uint64_t n_runs, void* stream) {
     if (!src || !dst) return fail(HS_E_ARG, "null KV region");
-    if (std::memcmp(&src->spec, &dst->spec, sizeof(hs_kv_spec)) != 0)
+    if (std::memcmp(&src->spec, &dst->spec, sizeof(hs_kv_spec)) != 0 || src->block8 != dst->block8)
         return fail(HS_E_ARG, "KV specs differ between source and destination");
     uint64_t total;
     int rc = check_runs(runs, n_runs, src->bytes, &total);
@@ -1641,6 +1691,14 @@ int hs_scratch_nll(hs_scratch* s, uint32_t next, double* out) {
     HS_CUDA_TRY(cudaMemcpyAsync(out, s->nll, 8, cudaMemcpyDeviceToHost, s->st));
     HS_CUDA_TRY(cudaStreamSynchronize(s->st));
     return HS_OK;
+}
+
+int hs_scratch_logprobs(hs_scratch* s, uint32_t next, uint32_t top, float* logp, float* entropy, uint32_t* rank,
+                        uint32_t* top_ids, float* top_logp) {
+    if (!s) return fail(HS_E_ARG, "null argument");
+    HS_CUDA_TRY(cudaSetDevice(s->m->device));
+    return scores_to_host(&s->scores, 1, s->logits, 1, s->m->cfg.vocab, &next, top, logp, entropy, rank, top_ids,
+                          top_logp, s->st);
 }
 
 int hs_scratch_set_logits(hs_scratch* s, const float* host, uint64_t n) {
@@ -1926,6 +1984,7 @@ struct hs_batch {
     float* wps = nullptr;
     double* nll = nullptr;         // perplexity scores of the last forward (hs_batch_nll) [cap_slots]
     uint32_t* nll_next = nullptr;
+    uint32_t* scores = nullptr;    // hs_batch_logprobs: tokens and scores of cap_slots rows
     uint32_t* err = nullptr;       // GEMM error word (device)
     uint32_t err_h = 0;
     float* sc_global = nullptr;    // attention scores for long contexts [cap_slots][nh][max_ctx]
@@ -1953,7 +2012,7 @@ struct hs_batch {
                         (void*)hb_hi, (void*)hb_lo, (void*)ctl, (void*)tokens, (void*)tok_tab, (void*)kv_tab,
                         (void*)dirty_tab, (void*)track_tab, (void*)cand, (void*)argbuf, (void*)err,
                         (void*)sc_global, (void*)att_part, (void*)att_cnt, (void*)sort_cand, (void*)wkeys,
-                        (void*)wps, (void*)nll, (void*)nll_next, (void*)pf_part})
+                        (void*)wps, (void*)nll, (void*)nll_next, (void*)scores, (void*)pf_part})
             cudaFree(p);
     }
 };
@@ -2376,6 +2435,15 @@ int hs_batch_nll(hs_batch* b, const uint32_t* next, uint32_t n, double* out) {
     HS_CUDA_TRY(cudaMemcpyAsync(out, b->nll, (size_t)n * 8, cudaMemcpyDeviceToHost, b->st));
     HS_CUDA_TRY(cudaStreamSynchronize(b->st));
     return HS_OK;
+}
+
+int hs_batch_logprobs(hs_batch* b, const uint32_t* next, uint32_t n, uint32_t top, float* logp, float* entropy,
+                      uint32_t* rank, uint32_t* top_ids, float* top_logp) {
+    if (!b) return fail(HS_E_ARG, "null argument");
+    if (n > b->cap_slots) return fail(HS_E_ARG, "more rows than the batch holds");
+    HS_CUDA_TRY(cudaSetDevice(b->m->device));
+    return scores_to_host(&b->scores, b->cap_slots, b->logits, n, b->m->cfg.vocab, next, top, logp, entropy, rank,
+                          top_ids, top_logp, b->st);
 }
 
 int hs_batch_logits(hs_batch* b, uint32_t slot, float* host, uint64_t n) {

@@ -102,6 +102,22 @@ cudaError_t launch_copy_runs(const uint8_t* src, uint8_t* dst, const XferRun* ru
 cudaError_t launch_logits_nll(const float* logits, uint64_t stride, const uint32_t* next, uint32_t rows,
                               uint32_t vocab, double* out, cudaStream_t st);
 
+// Scores of logit rows (logprobs.cu, hs_logprobs).
+constexpr uint32_t kLogprobTop = 64;  // largest `top`
+struct LogprobArgs {
+    const void* logits;
+    uint64_t row_stride;  // elements
+    uint32_t dtype, rows, vocab;
+    const uint32_t* ids;  // null: no logp, no rank
+    uint32_t top;
+    float *logp, *entropy;  // each output may be null
+    uint32_t *rank, *top_ids;
+    float* top_logp;
+};
+cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st);
+int check_logprobs(uint32_t rows, uint32_t vocab, const void* ids, uint32_t top, const void* logp, const void* rank,
+                   const void* top_ids, const void* top_logp);
+
 // Launchers (PDL attribute set; may be captured in a graph).
 cudaError_t launch_gemv(const GemvPlan& p, const GemvArgs& a, cudaStream_t st);
 cudaError_t launch_attention(uint32_t head_dim, uint32_t nh, size_t smem, const AttnArgs& a, cudaStream_t st);

@@ -1,0 +1,136 @@
+// The 8-bit KV cache: int8 codes with one f32 scale for each block of
+// `block` positions, each KV head, K and V apart (value = code * scale).
+//
+// Bytes of a region, layer after layer:
+//     K codes | V codes | K scales | V scales
+// each plane padded to 256 bytes. Code rows are head_dim bytes, [pos][head]
+// or [head][pos] by the region's layout; scales are [block][head] or
+// [head][block] accordingly.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.h"
+
+namespace hs {
+
+constexpr uint32_t kKv8MaxBlock = 128;
+constexpr uint32_t kPosNone = 0xffffffffu;  // HS_POS_NONE
+
+struct Kv8Geo {
+    uint64_t plane = 0, splane = 0, layers = 0;  // bytes of a code plane, of a scale plane
+    __host__ __device__ uint64_t layer_bytes() const { return 2 * (plane + splane); }
+    uint64_t bytes() const { return layers * layer_bytes(); }
+};
+inline Kv8Geo kv8_geo(const hs_kv_spec& s, uint32_t block) {
+    auto pad = [](uint64_t v) { return (v + 255) / 256 * 256; };
+    Kv8Geo g;
+    g.layers = s.n_layers;
+    g.plane = pad((uint64_t)s.max_ctx * s.n_kv_heads * s.head_dim);
+    g.splane = pad((uint64_t)((s.max_ctx + block - 1) / block) * s.n_kv_heads * 4);
+    return g;
+}
+// A shape that the 8-bit kernels take: HS_OK or an error.
+int kv8_check_shape(const hs_kv_spec& s, uint32_t block);
+
+// One layer of n regions as the kernels see it.
+struct Kv8View {
+    float* const* base = nullptr;             // per slot (device table)
+    uint64_t* const* dirty = nullptr;
+    const uint32_t* const* tracking = nullptr;
+    uint64_t layer_off = 0, plane = 0, splane = 0;
+    uint64_t pos_stride = 0, head_stride = 0;    // codes, bytes
+    uint64_t sblk_stride = 0, shead_stride = 0;  // scales, elements
+    uint32_t n_slots = 0, nkv = 0, max_ctx = 0, block_shift = 0, page_shift = 0;
+
+    __device__ uint64_t code_off(uint32_t v, uint32_t head, uint32_t pos) const {
+        return layer_off + (v ? plane : 0) + (uint64_t)pos * pos_stride + (uint64_t)head * head_stride;
+    }
+    __device__ uint64_t scale_off(uint32_t v, uint32_t head, uint32_t blk) const {
+        return layer_off + 2 * plane + (v ? splane : 0) +
+               ((uint64_t)blk * sblk_stride + (uint64_t)head * shead_stride) * 4;
+    }
+};
+inline Kv8View kv8_view(const hs_kv_spec& s, uint32_t block, uint32_t layer) {
+    const Kv8Geo g = kv8_geo(s, block);
+    Kv8View v;
+    v.layer_off = layer * g.layer_bytes();
+    v.plane = g.plane;
+    v.splane = g.splane;
+    const uint64_t hd = s.head_dim, nb = (s.max_ctx + block - 1) / block;
+    v.pos_stride = s.layout == HS_LAYOUT_TOKEN_MAJOR ? s.n_kv_heads * hd : hd;
+    v.head_stride = s.layout == HS_LAYOUT_TOKEN_MAJOR ? hd : (uint64_t)s.max_ctx * hd;
+    v.sblk_stride = s.layout == HS_LAYOUT_TOKEN_MAJOR ? s.n_kv_heads : 1;
+    v.shead_stride = s.layout == HS_LAYOUT_TOKEN_MAJOR ? 1 : nb;
+    v.nkv = s.n_kv_heads;
+    v.max_ctx = s.max_ctx;
+    v.block_shift = (uint32_t)__builtin_ctz(block);
+    return v;
+}
+
+// Rows of a ragged batch: slot i's are row_start[i] .. row_start[i + 1] - 1
+// (row_start null: row i alone), at positions pos[i], pos[i] + 1, ...
+struct Kv8Rows {
+    uint32_t n_rows = 0, n_slots = 0;
+    const uint32_t* row_start = nullptr;
+    const uint32_t* pos = nullptr;
+    uint32_t* err = nullptr;  // ERR_POS is set here for rows past max_ctx
+};
+
+// Element types of rows (HS_F32, HS_F16, HS_BF16) with their strides in
+// elements; a row's head_dim elements are consecutive.
+struct Kv8Mat {
+    const void* p = nullptr;
+    uint64_t row = 0, head = 0;
+    uint32_t dtype = 0;
+};
+inline uint32_t dtype_bytes(uint32_t dtype) { return dtype == HS_F32 ? 4 : 2; }
+
+cudaError_t launch_kv8_append(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows, const Kv8Mat& k, const Kv8Mat& v,
+                              cudaStream_t st);
+cudaError_t launch_kv8_read(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows, const Kv8Mat& k, const Kv8Mat& v,
+                            cudaStream_t st);
+
+struct Kv8AttendArgs {
+    Kv8View kv;
+    Kv8Rows rows;
+    Kv8Mat q, out;
+    uint32_t nh = 0;
+    float scale = 1.0f;
+};
+cudaError_t launch_kv8_attend(uint32_t hd, const Kv8AttendArgs& a, cudaStream_t st);
+
+#ifdef __CUDACC__
+// Row `r` of the batch: its slot and position. False for a row that is not
+// there (behind the last sequence, no position, or past max_ctx: flagged).
+__device__ __forceinline__ uint32_t kv8_slot_of(const Kv8Rows& rows, uint32_t r) {
+    if (!rows.row_start) return r;
+    uint32_t lo = 0, hi = rows.n_slots;  // the last slot whose first row is <= r and that is not empty
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (__ldg(rows.row_start + mid + 1) <= r)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    return lo;  // n_slots: behind the last sequence
+}
+__device__ __forceinline__ bool kv8_place(const Kv8Rows& rows, uint32_t max_ctx, uint32_t r, uint32_t* slot,
+                                          uint32_t* pos) {
+    const uint32_t s = kv8_slot_of(rows, r);
+    if (s >= rows.n_slots) return false;
+    const uint32_t first = rows.row_start ? __ldg(rows.row_start + s) : r, p0 = __ldg(rows.pos + s);
+    if (p0 == kPosNone || first > r) return false;
+    const uint64_t p = (uint64_t)p0 + (r - first);
+    if (p >= max_ctx) {
+        atomicOr(rows.err, 4u /* ERR_POS */);
+        return false;
+    }
+    *slot = s;
+    *pos = (uint32_t)p;
+    return true;
+}
+#endif
+
+}  // namespace hs

@@ -79,10 +79,10 @@ namespace {
 
 int live_runs(const hs_migration* g, const uint64_t* words, uint64_t from, uint64_t to, std::vector<uint64_t>* runs) {
     std::vector<uint64_t> live(2 * (size_t)(2 * g->spec.n_layers * g->spec.n_kv_heads + 2));
-    uint64_t n_live = hs_kv_live_ranges_between(&g->spec, (uint32_t)from, (uint32_t)to, live.data(), live.size() / 2);
+    uint64_t n_live = hs::kv_live_ranges(g->src, (uint32_t)from, (uint32_t)to, live.data(), live.size() / 2);
     if (n_live > live.size() / 2) {
         live.resize(2 * n_live);
-        n_live = hs_kv_live_ranges_between(&g->spec, (uint32_t)from, (uint32_t)to, live.data(), n_live);
+        n_live = hs::kv_live_ranges(g->src, (uint32_t)from, (uint32_t)to, live.data(), n_live);
     }
     runs->assign(2 * (size_t)std::max<uint64_t>(n_live, 1) + 2, 0);
     uint64_t n = hs_runs_to_byte_runs(words, g->n_pages, g->page_size, live.data(), n_live, runs->data(),
@@ -165,6 +165,9 @@ int hs_migrate_begin(hs_kv* src, hs_kv* dst, const hs_migrate_opts* opts, uint64
         return fail(HS_E_STATE, m);
     }
     if (std::memcmp(&ds, &g->spec, sizeof ds) != 0) return fail(HS_E_STATE, "destination refused: KV spec mismatch");
+    uint32_t bs = 0, bd = 0;
+    if ((rc = hs_kv8_block(src, &bs)) || (rc = hs_kv8_block(dst, &bd))) return rc;
+    if (bs != bd) return fail(HS_E_STATE, "destination refused: KV cache format mismatch");
     if (dpage != g->page_size) return fail(HS_E_STATE, "destination refused: page size mismatch");
     if (filled >= g->spec.max_ctx || upper < filled) return fail(HS_E_ARG, "filled past max_ctx or above upper");
     g->n_words = (g->n_pages + 63) / 64;
@@ -274,8 +277,8 @@ int hs_migrate_finish(hs_migration* g, uint64_t filled, uint64_t tokens_total, d
     }
     r.dest_resume_us = us_since(t_dest);
     r.stw_us = us_since(t_parked) + park_us;
-    std::vector<uint64_t> live(2 * (size_t)(2 * g->spec.n_layers * g->spec.n_kv_heads + 2));
-    uint64_t n_live = hs_kv_live_ranges_between(&g->spec, 0, (uint32_t)filled, live.data(), live.size() / 2);
+    std::vector<uint64_t> live(2 * (size_t)(4 * g->spec.n_layers * g->spec.n_kv_heads + 2));
+    uint64_t n_live = hs::kv_live_ranges(g->src, 0, (uint32_t)filled, live.data(), live.size() / 2);
     r.live_bytes = 0;
     for (uint64_t i = 0; i < std::min<uint64_t>(n_live, live.size() / 2); i++) r.live_bytes += live[2 * i + 1];
     r.filled = filled;

@@ -207,6 +207,85 @@ uint64_t hs_kv_live_ranges_between(const hs_kv_spec* s, uint32_t from, uint32_t 
 uint64_t hs_runs_to_byte_runs(const uint64_t* words, uint64_t n_pages, uint64_t page_size, const uint64_t* live,
                               uint64_t n_live, uint64_t* out, uint64_t cap);
 
+/* ---- 8-bit KV cache ---------------------------------------------------------
+ * A region whose rows are int8 codes with one f32 scale for each block of
+ * `block` positions (1, 16, 32, 64 or 128), each KV head, K and V apart:
+ * value = code * scale. No counterpart in the reference, whose cache is f32;
+ * it holds a position in a quarter of the bytes, which every decode step
+ * reads and every hand-over sends. The hs_kv_* calls on bytes, pages, runs
+ * and hashes and hs_migrate_* take it as they take an f32 region (both ends
+ * of a hand-over must have the same format and block); hs_forward and
+ * hs_seq_* refuse it, hs_batch_* and hs_prefill decode over it on the
+ * tensor-core path.
+ *
+ * How rows are stored (the same bits on any GPU): need = max|x| times 1/127,
+ * both in f32, over the new rows of a block and head (0 if below 2^-126, NaN
+ * if a value is infinite or NaN: all values under it then read back as NaN). A block that
+ * these rows begin takes s = need; one that holds older rows keeps its scale
+ * s, doubled as often as s >= need takes (the older codes halve as often,
+ * rounded to nearest, ties to even; a scale of NaN stays). A code is the
+ * integer nearest to x / s, ties to even. A value is then within s / 2 of
+ * what was stored, and within s where its block's scale grew after it. With
+ * block 1 a row's bytes never change and do not depend on how a prompt was
+ * cut into calls. */
+#define HS_F32 0u
+#define HS_F16 1u
+#define HS_BF16 2u
+#define HS_POS_NONE 0xffffffffu
+int hs_kv8_alloc(int device, const hs_kv_spec* spec, uint32_t block, uint32_t page_size, uint64_t fingerprint,
+                 hs_kv** out);
+/* ... of a model's shape and fingerprint, as hs_kv_alloc. */
+int hs_kv8_alloc_model(const hs_model* m, uint32_t layout, uint32_t block, uint32_t page_size, hs_kv** out);
+int hs_kv8_open_ipc(const hs_model* m, const void* handle, uint32_t layout, uint32_t block, uint32_t page_size,
+                    hs_kv** out);
+/* The positions under one scale; 0 for an f32 region. */
+int hs_kv8_block(const hs_kv* kv, uint32_t* block);
+/* hs_kv_live_ranges_between of an 8-bit region: codes and scales, from the
+ * start of the block that holds `from` (its older codes change as it fills). */
+uint64_t hs_kv8_live_ranges_between(const hs_kv_spec* s, uint32_t block, uint32_t from, uint32_t to, uint64_t* out,
+                                    uint64_t cap);
+
+/* n 8-bit regions of one shape, block, page size and device, as the slots of
+ * batched calls: the device tables and the workspace of hs_kv8_attend for
+ * n_heads query heads (a multiple of the KV heads, at most 16 for each; 0: no
+ * attend). Like an hs_batch it is used by one call at a time: calls on one
+ * set, and replays of graphs captured from them, must follow one another (on
+ * one stream, or ordered by events). The regions must outlive it. */
+typedef struct hs_kv8_set hs_kv8_set;
+int hs_kv8_set_new(hs_kv* const* kvs, uint32_t n, uint32_t n_heads, hs_kv8_set** out);
+void hs_kv8_set_free(hs_kv8_set* s);
+/* Waits for `stream`, then HS_E_ARG if a call since the last check met a row
+ * past max_ctx (such rows are not stored, read or attended: outputs of read
+ * stay as they were, those of attend are zeros), and clears that. */
+int hs_kv8_set_check(hs_kv8_set* s, void* stream);
+
+/* The calls below enqueue on `stream` (a cudaStream_t of the set's device;
+ * NULL = the legacy default stream), do not wait, allocate nothing and can be
+ * captured. Their rows: slot i's are row_start[i] .. row_start[i + 1] - 1 of
+ * n_rows, at positions pos[i], pos[i] + 1, ...; row_start (n + 1 entries,
+ * ascending) and pos (n entries) are device memory read when the call runs;
+ * row_start NULL: one row for each slot (n_rows = n). A slot at HS_POS_NONE
+ * has no rows for append and read, and its rows see nothing in attend
+ * (zeros). Rows from row_start[n] on are left as they were. Matrices are
+ * device memory of type `dtype` with strides in elements; the head_dim
+ * elements of a row and head are consecutive. */
+
+/* Quantises rows of K and V into layer `layer` (and marks their pages). */
+int hs_kv8_append(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* row_start, const uint32_t* pos,
+                  const void* k, const void* v, uint32_t dtype, uint64_t row_stride, uint64_t head_stride,
+                  void* stream);
+/* The values of cached rows, each rounded once to `dtype`; k or v may be NULL. */
+int hs_kv8_read(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* row_start, const uint32_t* pos,
+                void* k, void* v, uint32_t dtype, uint64_t row_stride, uint64_t head_stride, void* stream);
+/* Causal attention: the row at position p of slot i attends positions 0..p of
+ * region i (so append its K and V first) with its n_heads query heads, query
+ * head h on KV head h / (n_heads / n_kv_heads): softmax(scale * q.k) . v.
+ * Statistics and sums are f32; a row's bits do not depend on the other slots
+ * of the batch. `out` must not overlap `q`. */
+int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* row_start, const uint32_t* pos,
+                  const void* q, uint64_t q_row_stride, uint64_t q_head_stride, void* out, uint64_t out_row_stride,
+                  uint64_t out_head_stride, uint32_t dtype, float scale, void* stream);
+
 /* ---- forward (replaces Model::scratch / Model::forward, model.rs:221-327) - */
 
 int hs_scratch_new(const hs_model* m, hs_scratch** out);
@@ -344,6 +423,32 @@ int hs_seq_launches_per_step(hs_scratch* s, uint32_t* out);
  * previous kernel, last CTA exit, last CTA entry, then four kernel-specific
  * checkpoints (latest CTA). *used = number of launch slots. */
 int hs_scratch_trace(hs_scratch* s, uint64_t* out, uint64_t n_slots, uint64_t* used);
+
+/* ---- scores of logits ---------------------------------------------------------
+ * For each of `rows` rows of `vocab` logits in device memory (type `dtype`,
+ * row_stride elements apart, the logits of a row consecutive), with Z the sum
+ * of exp(logit):
+ *   logp[r]    = logit[ids[r]] - ln Z                (NaN if ids[r] >= vocab)
+ *   entropy[r] = -sum p ln p, p = exp(logit) / Z
+ *   rank[r]    = how many tokens come before ids[r] in the order (logit
+ *                descending, id ascending); 0xffffffff if ids[r] >= vocab
+ *   top_ids, top_logp [rows][top]: that order's first `top` tokens (0..64,
+ *                at most vocab)
+ * Outputs and ids are device memory; each output may be NULL (ids too, then
+ * logp and rank must be). A logit of -inf is a token that cannot come (p = 0);
+ * a row of nothing else, one with +inf and one with NaN have logp, top_logp
+ * and entropy NaN (NaN logits come first in the order). Enqueued on `stream`
+ * (NULL = the legacy default stream) of `device`, not waited for; allocates
+ * nothing, keeps no state between calls. */
+int hs_logprobs(int device, const void* logits, uint32_t dtype, uint64_t row_stride, uint32_t rows, uint32_t vocab,
+                const uint32_t* ids, uint32_t top, float* logp, float* entropy, uint32_t* rank, uint32_t* top_ids,
+                float* top_logp, void* stream);
+/* The same of the scratch's logits, into host memory (one row). */
+int hs_scratch_logprobs(hs_scratch* s, uint32_t next, uint32_t top, float* logp, float* entropy, uint32_t* rank,
+                        uint32_t* top_ids, float* top_logp);
+/* ... of slots 0..n-1 of the last hs_forward_batch, into host memory. */
+int hs_batch_logprobs(hs_batch* b, const uint32_t* next, uint32_t n, uint32_t top, float* logp, float* entropy,
+                      uint32_t* rank, uint32_t* top_ids, float* top_logp);
 
 /* ---- load-time dequantisation as a standalone op (quant.rs:18-38) ------ */
 
