@@ -92,12 +92,32 @@ cudaError_t launch_kv8_append(uint32_t hd, const Kv8View& kv, const Kv8Rows& row
 cudaError_t launch_kv8_read(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows, const Kv8Mat& k, const Kv8Mat& v,
                             cudaStream_t st);
 
+// A single row's positions are split between CTAs by its own length and the
+// region's shape alone, so that its bits do not depend on the batch: 64 KB of
+// codes a split, and from about one CTA a KV head and SM (of a B200's 148) on
+// fewer, longer ones.
+constexpr uint32_t kv8_max_splits(uint32_t nkv) {
+    return nkv <= 1 ? 148 : 148 / nkv < 16 ? 16 : 148 / nkv;
+}
+__host__ __device__ constexpr uint32_t kv8_min_split(uint32_t hd) { return 32768 / hd; }
+__host__ __device__ inline uint32_t kv8_split_len(uint32_t n, uint32_t hd, uint32_t max_splits) {
+    const uint32_t len = ((n + max_splits - 1) / max_splits + 63) / 64 * 64, least = kv8_min_split(hd);
+    return len > least ? len : least;
+}
+// Query heads of one KV head that a CTA takes together.
+constexpr uint32_t kv8_single_cols(uint32_t group) { return group <= 8 ? 8 : 16; }
+
 struct Kv8AttendArgs {
     Kv8View kv;
     Kv8Rows rows;
     Kv8Mat q, out;
     uint32_t nh = 0;
     float scale = 1.0f;
+    // single rows: split records [slot][KV head][head chunk][split][cols x (head_dim + 2)]
+    // and, for each (slot, KV head, chunk), a counter that is zero between calls
+    float* part = nullptr;
+    uint32_t* counters = nullptr;
+    uint32_t max_splits = 0;
 };
 cudaError_t launch_kv8_attend(uint32_t hd, const Kv8AttendArgs& a, cudaStream_t st);
 
