@@ -6,9 +6,10 @@
 // other operand is an f16 pair hi + lo (22 bits) for f32 rows, one f16 for
 // 16-bit rows, after scaling by powers of two that keep it in f16's range:
 //   q:       its largest element to [2^13, 2^14)
-//   weights: w = exp(S - m) s_v 2^(14 - e), 2^e at or above the largest s_v so
-//            far, so that weights down to 2^-38 of the largest still count
+//   weights: w = exp(S - m) s_v 2^(10 - e), 2^e at or above the largest s_v so
+//            far, so that weights down to 2^-34 of the largest still count
 // Scores, statistics and sums are f32.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -16,6 +17,8 @@
 #include "device.cuh"
 #include "kernels.h"
 #include "kv8.h"
+
+namespace cg = cooperative_groups;
 
 namespace hs {
 namespace {
@@ -122,170 +125,219 @@ __device__ __forceinline__ float fit_f16(float amax, float* inverse) {
 }
 
 constexpr float kLog2e = 1.44269504088896341f;
-constexpr uint32_t kDecWarps = 4;
+// The running maximum of scores (in powers of two) is raised once a score
+// passes it by more than this: weights stay below 2^4, and most blocks skip
+// the reduction over the warp and the rescaling.
+constexpr float kSlack = 4.0f;
 
-// A single row per slot: one CTA takes a split of the positions of one
-// (slot, KV head), its warps blocks of BP positions in turn. A warp computes
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+
+// A single row per slot. One CTA takes a split of the positions of one (slot,
+// KV head), its warps blocks of BP positions in turn. A warp computes
 // S^T = K q^T (16 positions by 8 query heads an instruction; the codes are
 // the operand of 16 rows, so a group of up to 8 heads wastes none of it) and
 // O^T += V^T w^T, with K's and V's codes loaded straight into the operand
 // layout: a lane's 16 bytes of a K row are its share of four k-steps (a dot
 // product does not mind which), its bytes of four V rows its share of the
-// m-tiles. No code passes through shared memory.
+// m-tiles. Blocks arrive by cp.async in a ring of each warp's own, so that a
+// warp waits for its own copies only; with loads into registers instead, one
+// block ahead, the same kernel took 56 us (46) for 64 sequences of 8,192
+// positions, 14/2 heads of 64.
+//
+// The splits are joined in two levels: those of a cluster (up to 8) through
+// distributed shared memory, each CTA a share of the outputs; where a row has
+// more, each share's last cluster joins the clusters' records in order.
 template <int HD, int DT, int NT>
 struct DecGeom {
     static constexpr uint32_t BP = HD == 64 ? 32 : 16;  // positions of a block: 4 KB of codes either way
     static constexpr uint32_t MB = BP / 16;
     static constexpr uint32_t KS = HD / 16;             // k-steps of the scores, m-tiles of the output
-    static constexpr bool PAIR = DT == HS_F32;
     static constexpr uint32_t NC = 8 * NT;
-};
-
-template <int HD>
-struct DecBlock {  // codes and scales of BP positions as one lane holds them
-    static constexpr uint32_t MB = HD == 64 ? 2 : 1;
-    uint4 k[MB][2][HD / 64];   // K rows g and g + 8 of each 16: 16 bytes a 64-byte part
-    uint32_t v[MB][4][HD / 32];  // V rows 2t, 2t+1, 2t+8, 2t+9: HD / 8 bytes
-    float ks[MB][2], vs[MB][2];
+    static constexpr uint32_t W = 4, THREADS = 32 * W;
+    // A warp's ring of blocks: K rows; V rows, padded so that the rows a lane
+    // group reads together fall into different banks; K and V scales.
+    static constexpr uint32_t STAGES = 2, VP = HD + 16, V_AT = BP * HD, S_AT = V_AT + BP * VP, STAGE = S_AT + 8 * BP;
+    static constexpr uint32_t RING = W * STAGES * STAGE;
+    static constexpr uint32_t OS = HD + 4;  // row stride of the outputs, which take the ring's space
+    static_assert(RING >= W * NC * OS * 4, "the outputs fit in the ring");
+    // f32 rows keep q and the weights as pairs; f16 ones the weights (one f16
+    // would double their result's own rounding); q of 16 bits is exact in one
+    static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
 };
 
 template <int HD, int DT, int NT>
-__global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendArgs a) {
+__global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2) k_kv8_single(const Kv8AttendArgs a) {
     using G = DecGeom<HD, DT, NT>;
-    constexpr uint32_t BP = G::BP, MB = G::MB, KS = G::KS, NC = G::NC;
-    constexpr bool PAIR = G::PAIR;
-    __shared__ float sm_o[kDecWarps][NC][HD + 4];
-    __shared__ float sm_m[kDecWarps][NC], sm_l[kDecWarps][NC];
+    constexpr uint32_t BP = G::BP, MB = G::MB, KS = G::KS, NC = G::NC, W = G::W, THREADS = G::THREADS;
+    constexpr uint32_t OS = G::OS;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ uint32_t sm_q[2][NT][KS][2][32];  // q as operand words [hi, lo][k-step][2][lane]
+    __shared__ float sm_m[W][NC], sm_l[W][NC], sm_cf[NC], cta_m[NC], cta_l[NC];
     __shared__ uint32_t sm_last;
+    float(*sm_o)[NC][OS] = reinterpret_cast<float(*)[NC][OS]>(smem);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t group = a.nh / a.kv.nkv, chunks = (group + NC - 1) / NC;
-    const uint32_t item = blockIdx.x;
-    const uint32_t slot = item / (a.kv.nkv * chunks), rest = item - slot * a.kv.nkv * chunks;
-    const uint32_t kvh = rest / chunks, chunk = rest - kvh * chunks;
-    const uint32_t h0 = kvh * group + chunk * NC, cols = min(NC, group - chunk * NC);
-    const uint32_t split = blockIdx.y;
+    // KV heads of a position run side by side: with rows [pos][head] they share lines of the L2
+    const uint32_t slot = blockIdx.z, split = blockIdx.y, cs = a.cluster, first = split & ~(cs - 1);
+    const uint32_t kvh = a.chunks == 1 ? blockIdx.x : blockIdx.x / a.chunks, chunk = blockIdx.x - kvh * a.chunks;
+    const uint32_t h0 = kvh * a.group + chunk * NC, cols = min(NC, a.group - chunk * NC);
+    const uint32_t item = slot * gridDim.x + blockIdx.x;
     const uint32_t pos = __ldg(a.rows.pos + slot);
     const uint8_t* base = reinterpret_cast<const uint8_t*>(__ldg(reinterpret_cast<const unsigned long long*>(a.kv.base + slot)));
-    if (pos >= a.kv.max_ctx) {
+    if (pos >= a.kv.max_ctx) {  // the whole cluster leaves here
         if (split == 0) {
             if (pos != kPosNone && tid == 0) atomicOr(a.rows.err, ERR_POS);
-            for (uint32_t i = tid; i < cols * HD; i += kDecWarps * 32)
+            for (uint32_t i = tid; i < cols * HD; i += THREADS)
                 store1<DT>(const_cast<void*>(a.out.p), slot * a.out.row + (h0 + i / HD) * a.out.head + i % HD, 0.0f);
         }
         return;
     }
-    const uint32_t n = pos + 1, len = kv8_split_len(n, HD, a.max_splits), splits = (n + len - 1) / len;
-    if (split >= splits) return;
-    const uint32_t from = split * len, to = min(n, from + len);
+    const uint32_t n = pos + 1;
+    const uint32_t len = kv8_split_len(n, HD, a.max_splits), splits = (n + len - 1) / len;
+    // and here: no split for this CTA, in a cluster that has none or that joins
+    // without it (a thread that has left is not waited for at a cluster's barrier)
+    if (split >= splits && (first >= splits || splits <= cs)) return;
+    const uint32_t from = min(split * len, n), to = min(n, from + len);
 
-    const uint8_t* kp = base + a.kv.code_off(0, kvh, 0);
-    const uint8_t* vp = base + a.kv.code_off(1, kvh, 0);
+    const uint64_t ps = a.kv.pos_stride;
     const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, 0));
     const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, 0));
-    const uint64_t ps = a.kv.pos_stride;
+    constexpr uint32_t LPR = HD / 16, RPI = 32 / LPR;  // lanes a row, rows a warp copies at once
+    const uint32_t lr = lane / LPR, lc = lane % LPR * 16;
+    const uint8_t* kp = base + a.kv.code_off(0, kvh, 0) + lc;
+    const uint8_t* vp = base + a.kv.code_off(1, kvh, 0) + lc;
+    uint8_t* ring = smem + warp * (G::STAGES * G::STAGE);
 
-    // Positions past the split are read as its last one and get no weight.
-    DecBlock<HD> buf;
-    auto load = [&](uint32_t p0) {
+    // Copies the block at p0 into a stage. Positions past the split are read
+    // as its last one and get no weight. One group a call, empty past the end.
+    auto fetch = [&](uint32_t p0, uint8_t* st) {
+        if (p0 < to) {
+            const uint64_t sp = (uint64_t)(min(p0 + lane % BP, to - 1) >> a.kv.block_shift) * a.kv.sblk_stride;
+            if (HD == 64 || lane < 16) cp_async4(st + G::S_AT + 4 * (lane % BP), ksp + sp);
+            if (HD == 64 || lane >= 16) cp_async4(st + G::S_AT + 4 * BP + 4 * (lane % BP), vsp + sp);
+            uint8_t *dk = st + lr * HD + lc, *dv = st + G::V_AT + lr * G::VP + lc;
+            if (p0 + BP <= to) {
+                const uint64_t at = (p0 + lr) * ps, step = RPI * ps;
+                const uint8_t *k = kp + at, *v = vp + at;
 #pragma unroll
-        for (uint32_t b = 0; b < MB; b++) {
+                for (uint32_t i = 0; i < BP / RPI; i++, k += step, v += step) {
+                    cp_async16(dk + i * RPI * HD, k);
+                    cp_async16(dv + i * RPI * G::VP, v);
+                }
+            } else {
 #pragma unroll
-            for (uint32_t r = 0; r < 2; r++) {
-                const uint32_t p = min(p0 + 16 * b + 8 * r + g, to - 1);
-#pragma unroll
-                for (uint32_t c = 0; c < HD / 64; c++)
-                    buf.k[b][r][c] = __ldg(reinterpret_cast<const uint4*>(kp + p * ps + 64 * c + 16 * t));
-                buf.ks[b][r] = __ldg(ksp + (p >> a.kv.block_shift) * a.kv.sblk_stride);
-                buf.vs[b][r] = __ldg(vsp + (p >> a.kv.block_shift) * a.kv.sblk_stride);
-            }
-#pragma unroll
-            for (uint32_t r = 0; r < 4; r++) {
-                const uint32_t p = min(p0 + 16 * b + 2 * t + (r & 1) + 8 * (r >> 1), to - 1);
-                const uint8_t* q = vp + p * ps + (HD / 8) * g;
-                if constexpr (HD == 64) {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
-                    buf.v[b][r][0] = w.x, buf.v[b][r][1] = w.y;
-                } else {
-                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(q));
-                    buf.v[b][r][0] = w.x, buf.v[b][r][1] = w.y, buf.v[b][r][2] = w.z, buf.v[b][r][3] = w.w;
+                for (uint32_t i = 0; i < BP / RPI; i++) {
+                    const uint64_t at = min(p0 + lr + i * RPI, to - 1) * ps;
+                    cp_async16(dk + i * RPI * HD, kp + at);
+                    cp_async16(dv + i * RPI * G::VP, vp + at);
                 }
             }
         }
+        cp_async_commit();
     };
-    uint32_t p0 = from + warp * BP;
-    if (p0 < to) load(p0);
+    uint32_t p0 = from + warp * BP, st_in = 0, st_out = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < G::STAGES - 1; i++) fetch(p0 + i * W * BP, ring + i * G::STAGE);
+    st_in = G::STAGES - 1;
 
-    // q as the second operand: column g of n-tile nt is head h0 + 8 nt + g
-    uint32_t qh[NT][KS][2], ql[PAIR ? NT : 1][PAIR ? KS : 1][2];
+    // q as the second operand, prepared once for the CTA: column c of n-tile
+    // c / 8 is head h0 + c, its element d = 64 i + 16 t + 4 j + e goes to k-step
+    // 4 i + j of lane 4 (c % 8) + t: word e % 2, half e / 2
+#pragma unroll
+    for (uint32_t i = 0; i < NC / W; i++) {
+        const uint32_t c = warp * (NC / W) + i;
+        float x[HD / 32], top = 0.0f;
+#pragma unroll
+        for (uint32_t e = 0; e < HD / 32; e++) {
+            x[e] = c < cols ? load1<DT>(a.q.p, slot * a.q.row + (uint64_t)(h0 + c) * a.q.head + lane + 32 * e) : 0.0f;
+            top = fmaxf(top, fabsf(x[e]));
+        }
+#pragma unroll
+        for (uint32_t d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        float inv;
+        const float fit = fit_f16(top, &inv);
+        if (lane == 0) sm_cf[c] = (a.scale * kLog2e) * inv;
+#pragma unroll
+        for (uint32_t e = 0; e < HD / 32; e++) {
+            const uint32_t d = lane + 32 * e, k = d / 64 * 4 + d % 16 / 4, to_lane = 4 * (c % 8) + d % 64 / 16;
+            const __half hi = __float2half_rn(x[e] * fit);
+            reinterpret_cast<__half*>(&sm_q[0][c / 8][k][d & 1][to_lane])[(d & 2) / 2] = hi;
+            if constexpr (G::QPAIR)
+                reinterpret_cast<__half*>(&sm_q[1][c / 8][k][d & 1][to_lane])[(d & 2) / 2] =
+                    __float2half_rn(x[e] * fit - __half2float(hi));
+        }
+    }
+    __syncthreads();
+    uint32_t qh[NT][KS][2], ql[G::QPAIR ? NT : 1][G::QPAIR ? KS : 1][2];
     float cf[NT][2];  // columns 2t, 2t + 1: softmax scale x log2(e) x what q was scaled by
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; nt++) {
-        float x[HD / 4], top = 0.0f;
-        const uint32_t col = 8 * nt + g;
+        cf[nt][0] = sm_cf[8 * nt + 2 * t], cf[nt][1] = sm_cf[8 * nt + 2 * t + 1];
 #pragma unroll
-        for (uint32_t i = 0; i < HD / 4; i++) {
-            x[i] = col < cols ? load1<DT>(a.q.p, slot * a.q.row + (uint64_t)(h0 + col) * a.q.head + (i / 16) * 64 + 16 * t + i % 16) : 0.0f;
-            top = fmaxf(top, fabsf(x[i]));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        float inv;
-        const float fit = fit_f16(top, &inv);
-        const float back = (a.scale * kLog2e) * inv;
-        cf[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);
-        cf[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+        for (uint32_t j = 0; j < KS; j++)
 #pragma unroll
-        for (uint32_t j = 0; j < KS; j++) {
-            const float* e = x + 4 * j;
-            if constexpr (PAIR) {
-                pair16(e[0] * fit, e[2] * fit, &qh[nt][j][0], &ql[nt][j][0]);
-                pair16(e[1] * fit, e[3] * fit, &qh[nt][j][1], &ql[nt][j][1]);
-            } else {
-                const __half2 u = __floats2half2_rn(e[0] * fit, e[2] * fit), v = __floats2half2_rn(e[1] * fit, e[3] * fit);
-                qh[nt][j][0] = *reinterpret_cast<const uint32_t*>(&u);
-                qh[nt][j][1] = *reinterpret_cast<const uint32_t*>(&v);
+            for (uint32_t w = 0; w < 2; w++) {
+                qh[nt][j][w] = sm_q[0][nt][j][w][lane];
+                if constexpr (G::QPAIR) ql[nt][j][w] = sm_q[1][nt][j][w][lane];
             }
-        }
     }
 
     float o[NT][KS][4] = {}, m[NT][2], l[NT][2] = {}, vmax = 0.0f, vfit = 0.0f;
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
 
-    for (; p0 < to; p0 += kDecWarps * BP) {
+    auto block = [&](auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        cp_async_wait<G::STAGES - 2>();
+        __syncwarp();
+        const uint8_t* st = ring + st_out * G::STAGE;
+        st_out = st_out + 1 == G::STAGES ? 0 : st_out + 1;
+        // the stage before this one was read to its end: its space takes the next block
+        fetch(p0 + (G::STAGES - 1) * W * BP, ring + st_in * G::STAGE);
+        st_in = st_in + 1 == G::STAGES ? 0 : st_in + 1;
         // scores: rows g and g + 8 of each 16 positions, columns 2t and 2t + 1
         float s[NT][MB][4] = {};
 #pragma unroll
         for (uint32_t b = 0; b < MB; b++)
 #pragma unroll
             for (uint32_t j = 0; j < KS; j++) {
-                const uint4 w0 = buf.k[b][0][j / 4], w1 = buf.k[b][1][j / 4];
+                const uint4 w0 = *reinterpret_cast<const uint4*>(st + (16 * b + g) * HD + j / 4 * 64 + 16 * t);
+                const uint4 w1 = *reinterpret_cast<const uint4*>(st + (16 * b + 8 + g) * HD + j / 4 * 64 + 16 * t);
                 const uint32_t u = j % 4 == 0 ? w0.x : j % 4 == 1 ? w0.y : j % 4 == 2 ? w0.z : w0.w;
                 const uint32_t v = j % 4 == 0 ? w1.x : j % 4 == 1 ? w1.y : j % 4 == 2 ? w1.z : w1.w;
                 const uint32_t f[4] = {even_bytes(u), even_bytes(v), odd_bytes(u), odd_bytes(v)};
 #pragma unroll
                 for (uint32_t nt = 0; nt < NT; nt++) {
-                    if constexpr (PAIR) mma16816(s[nt][b], f, ql[nt][j][0], ql[nt][j][1]);
+                    if constexpr (G::QPAIR) mma16816(s[nt][b], f, ql[nt][j][0], ql[nt][j][1]);
                     mma16816(s[nt][b], f, qh[nt][j][0], qh[nt][j][1]);
                 }
             }
         float vs[MB][2], top[NT][2];
         bool grew = false, vgrew = false;
 #pragma unroll
-        for (uint32_t nt = 0; nt < NT; nt++) top[nt][0] = m[nt][0], top[nt][1] = m[nt][1];
+        for (uint32_t nt = 0; nt < NT; nt++) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
         for (uint32_t b = 0; b < MB; b++)
 #pragma unroll
             for (uint32_t r = 0; r < 2; r++) {
-                const bool in = p0 + 16 * b + 8 * r + g < to;
-                vs[b][r] = in ? buf.vs[b][r] : 0.0f;
+                const uint32_t at = 16 * b + 8 * r + g;
+                const bool in = !TAIL || p0 + at < to;
+                const float ks = reinterpret_cast<const float*>(st + G::S_AT)[at];
+                vs[b][r] = in ? reinterpret_cast<const float*>(st + G::S_AT)[BP + at] : 0.0f;
                 vgrew |= vs[b][r] > vmax;
 #pragma unroll
                 for (uint32_t nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (uint32_t c = 0; c < 2; c++) {
                         float& x = s[nt][b][2 * r + c];
-                        x = in ? x * (buf.ks[b][r] * cf[nt][c]) : -INFINITY;
+                        x = in ? x * (ks * cf[nt][c]) : -INFINITY;
                         top[nt][c] = fmaxf(top[nt][c], x);
                     }
             }
@@ -293,18 +345,29 @@ __global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendAr
 #pragma unroll
         for (uint32_t b = 0; b < MB; b++)
 #pragma unroll
-            for (uint32_t i = 0; i < KS / 2; i++)
+            for (uint32_t h = 0; h < 2; h++) {
+                const uint8_t* v0 = st + G::V_AT + (16 * b + 8 * h + 2 * t) * G::VP + (HD / 8) * g;
+                uint32_t w[2][HD / 32];
 #pragma unroll
-                for (uint32_t h = 0; h < 2; h++) {
-                    const uint32_t w0 = buf.v[b][2 * h][i], w1 = buf.v[b][2 * h + 1][i];
-                    const uint32_t lo = __byte_perm(w0, w1, 0x5410), hi = __byte_perm(w0, w1, 0x7632);
+                for (uint32_t r = 0; r < 2; r++) {
+                    if constexpr (HD == 64) {
+                        const uint2 x = *reinterpret_cast<const uint2*>(v0 + r * G::VP);
+                        w[r][0] = x.x, w[r][1] = x.y;
+                    } else {
+                        const uint4 x = *reinterpret_cast<const uint4*>(v0 + r * G::VP);
+                        w[r][0] = x.x, w[r][1] = x.y, w[r][2] = x.z, w[r][3] = x.w;
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < KS / 2; i++) {
+                    const uint32_t lo = __byte_perm(w[0][i], w[1][i], 0x5410), hi = __byte_perm(w[0][i], w[1][i], 0x7632);
                     va[b][2 * i][2 * h] = even_bytes(lo), va[b][2 * i][2 * h + 1] = odd_bytes(lo);
                     va[b][2 * i + 1][2 * h] = even_bytes(hi), va[b][2 * i + 1][2 * h + 1] = odd_bytes(hi);
                 }
-        if (p0 + kDecWarps * BP < to) load(p0 + kDecWarps * BP);
+            }
 
 #pragma unroll
-        for (uint32_t nt = 0; nt < NT; nt++) grew |= top[nt][0] > m[nt][0] || top[nt][1] > m[nt][1];
+        for (uint32_t nt = 0; nt < NT; nt++) grew |= top[nt][0] > m[nt][0] + kSlack || top[nt][1] > m[nt][1] + kSlack;
         if (__any_sync(0xffffffffu, grew || vgrew)) {
             // new maxima for the warp (over the 8 row groups), older sums scaled to them
             float vnew = vmax;
@@ -313,9 +376,9 @@ __global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendAr
 #pragma unroll
             for (uint32_t d = 4; d < 32; d <<= 1) vnew = fmaxf(vnew, __shfl_xor_sync(0xffffffffu, vnew, d));
             float vback = 1.0f;
-            if (vnew > vmax) {  // the power of two above vnew, unless it is held already
+            if (vnew > vmax) {  // the power of two above vnew
                 const uint32_t e = min((__float_as_uint(vnew) >> 23) + 1, 254u);
-                const float fit = __uint_as_float(min(268u - e, 254u) << 23);  // largest weight 2^14
+                const float fit = __uint_as_float(min(264u - e, 254u) << 23);  // 2^10 for a weight of 1
                 vback = vfit > 0.0f ? fit / vfit : 1.0f;
                 vfit = fit;
                 vmax = __uint_as_float(e << 23);
@@ -324,7 +387,7 @@ __global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendAr
             for (uint32_t nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (uint32_t c = 0; c < 2; c++) {
-                    float x = top[nt][c];
+                    float x = fmaxf(m[nt][c], top[nt][c]);
 #pragma unroll
                     for (uint32_t d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     const float f = x == m[nt][c] ? 1.0f : ex2(m[nt][c] - x);
@@ -348,20 +411,24 @@ __global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendAr
                     l[nt][e & 1] += p;
                     w[e] = p * (vs[b][e >> 1] * vfit);
                 }
-                uint32_t h0, h1, l0 = 0, l1 = 0;
-                pair16(w[0], w[1], &h0, &l0);
-                pair16(w[2], w[3], &h1, &l1);
-                h0 = transpose8x8(h0), h1 = transpose8x8(h1);
-                if constexpr (PAIR) l0 = transpose8x8(l0), l1 = transpose8x8(l1);
+                uint32_t w0, w1, x0 = 0, x1 = 0;
+                pair16(w[0], w[1], &w0, &x0);
+                pair16(w[2], w[3], &w1, &x1);
+                w0 = transpose8x8(w0), w1 = transpose8x8(w1);
+                if constexpr (G::WPAIR) x0 = transpose8x8(x0), x1 = transpose8x8(x1);
 #pragma unroll
                 for (uint32_t i = 0; i < KS; i++) {
-                    if constexpr (PAIR) mma16816(o[nt][i], va[b][i], l0, l1);
-                    mma16816(o[nt][i], va[b][i], h0, h1);
+                    if constexpr (G::WPAIR) mma16816(o[nt][i], va[b][i], x0, x1);
+                    mma16816(o[nt][i], va[b][i], w0, w1);
                 }
             }
-    }
+    };
+    for (; p0 + BP <= to; p0 += W * BP) block(std::false_type{});
+    if (p0 < to) block(std::true_type{});
+    cp_async_wait<0>();
+    __syncthreads();  // every warp's ring is free for the outputs
 
-    // the warps' records, then the CTA's
+    // the warps' records: outputs [column][d], maxima and sums (a warp without a block: -inf, 0, 0)
     const float vinv = vfit > 0.0f ? 1.0f / vfit : 0.0f;
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; nt++)
@@ -372,56 +439,114 @@ __global__ void __launch_bounds__(kDecWarps * 32) k_kv8_single(const Kv8AttendAr
             for (uint32_t d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
             const uint32_t col = 8 * nt + 2 * t + c;
             if (g == 0) sm_m[warp][col] = m[nt][c], sm_l[warp][col] = x;
+            float* to_o = &sm_o[warp][col][(HD / 8) * g];
 #pragma unroll
-            for (uint32_t i = 0; i < KS; i++) {
-                sm_o[warp][col][(HD / 8) * g + 2 * i] = o[nt][i][c] * vinv;
-                sm_o[warp][col][(HD / 8) * g + 2 * i + 1] = o[nt][i][2 + c] * vinv;
-            }
+            for (uint32_t i = 0; i < KS; i += 2)
+                *reinterpret_cast<float4*>(to_o + 2 * i) = make_float4(o[nt][i][c] * vinv, o[nt][i][2 + c] * vinv,
+                                                                       o[nt][i + 1][c] * vinv, o[nt][i + 1][2 + c] * vinv);
         }
     __syncthreads();
-    constexpr uint32_t TH = kDecWarps * 32;
-    float* rec = a.part + (((uint64_t)item * a.max_splits + split) * NC) * (HD + 2);
-    for (uint32_t i = tid; i < cols * HD; i += TH) {
-        const uint32_t col = i / HD, d = i % HD;
-        float mm = -INFINITY, ll = 0.0f, acc = 0.0f;
+    // the CTA's record, in the first warp's place: a float4 of a column a thread
+    for (uint32_t i = tid; i < cols * (HD / 4); i += THREADS) {
+        const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f, f[W];
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (uint32_t w = 0; w < kDecWarps; w++) mm = fmaxf(mm, sm_m[w][col]);
+        for (uint32_t w = 0; w < W; w++) mm = fmaxf(mm, sm_m[w][col]);
 #pragma unroll
-        for (uint32_t w = 0; w < kDecWarps; w++) {
-            if (from + w * BP >= to) break;  // warps without a block
-            const float f = ex2(sm_m[w][col] - mm);
-            ll = fmaf(sm_l[w][col], f, ll);
-            acc = fmaf(sm_o[w][col][d], f, acc);
+        for (uint32_t w = 0; w < W; w++) {
+            f[w] = from + w * BP < to ? ex2(sm_m[w][col] - mm) : 0.0f;
+            ll = fmaf(sm_l[w][col], f[w], ll);
+            const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][col][d]);
+            acc.x = fmaf(x.x, f[w], acc.x), acc.y = fmaf(x.y, f[w], acc.y);
+            acc.z = fmaf(x.z, f[w], acc.z), acc.w = fmaf(x.w, f[w], acc.w);
         }
-        if (splits == 1) {
-            store1<DT>(const_cast<void*>(a.out.p), slot * a.out.row + (uint64_t)(h0 + col) * a.out.head + d, acc / ll);
+        *reinterpret_cast<float4*>(&sm_o[0][col][d]) = acc;
+        if (d == 0) cta_m[col] = mm, cta_l[col] = ll;
+    }
+    auto store = [&](uint32_t col, uint32_t d, float4 acc, float ll) {
+        const uint64_t at = slot * a.out.row + (uint64_t)(h0 + col) * a.out.head + d;
+        const float inv = __frcp_rn(ll);
+        store1<DT>(const_cast<void*>(a.out.p), at, acc.x * inv);
+        store1<DT>(const_cast<void*>(a.out.p), at + 1, acc.y * inv);
+        store1<DT>(const_cast<void*>(a.out.p), at + 2, acc.z * inv);
+        store1<DT>(const_cast<void*>(a.out.p), at + 3, acc.w * inv);
+    };
+    if (splits == 1) {
+        __syncthreads();
+        for (uint32_t i = tid; i < cols * (HD / 4); i += THREADS) {
+            const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
+            store(col, d, *reinterpret_cast<const float4*>(&sm_o[0][col][d]), cta_l[col]);
+        }
+        return;
+    }
+
+    // a cluster's splits: CTA `rank` joins its share of the outputs
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    const uint32_t rank = split - first, held = min(cs, splits - first);
+    const uint32_t shares = splits <= cs ? splits : cs;
+    const uint32_t per = (cols * (HD / 4) + shares - 1) / shares, i0 = rank * per, i1 = min(cols * (HD / 4), i0 + per);
+    const uint32_t n_cl = (splits + cs - 1) / cs;
+    constexpr uint32_t REC = kv8_record(HD, NC);  // outputs, then each share's copy of maxima and sums
+    float* rec0 = a.part + (uint64_t)item * a.max_clusters * REC;
+    float* rec = rec0 + first / cs * REC;
+    const uint32_t stats = NC * HD + rank * 2 * NC;
+    for (uint32_t i = i0 + tid; i < i1; i += THREADS) {
+        const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float mr[8];
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+            mr[r] = r < held ? *cl.map_shared_rank(&cta_m[col], r) : -INFINITY;
+            mm = fmaxf(mm, mr[r]);
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+            if (r >= held) continue;
+            const float f = ex2(mr[r] - mm);
+            ll = fmaf(*cl.map_shared_rank(&cta_l[col], r), f, ll);
+            const float4 x = *reinterpret_cast<const float4*>(cl.map_shared_rank(&sm_o[0][col][d], r));
+            acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
+            acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+        }
+        if (n_cl == 1) {
+            store(col, d, acc, ll);
         } else {
-            rec[i] = acc;
-            if (d == 0) rec[NC * HD + col] = mm, rec[NC * HD + NC + col] = ll;
+            *reinterpret_cast<float4*>(rec + 4 * i) = acc;
+            if (d == 0 || i == i0) rec[stats + col] = mm, rec[stats + NC + col] = ll;
         }
     }
-    if (splits == 1) return;
-    // the last CTA of this (slot, KV head, chunk) joins the splits in order
+    // no CTA leaves while others read its record
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+    if (n_cl == 1) return;
+
+    // more clusters: the last one to finish this share joins their records in order
     __threadfence();
     __syncthreads();
-    if (tid == 0) sm_last = atomicAdd(a.counters + item, 1u);
+    uint32_t* counter = a.counters + item * 8 + rank;
+    if (tid == 0) sm_last = atomicAdd(counter, 1u);
     __syncthreads();
-    if (sm_last != splits - 1) return;
+    if (sm_last != n_cl - 1) return;
     __threadfence();
-    if (tid == 0) a.counters[item] = 0;
-    const float* r0 = a.part + ((uint64_t)item * a.max_splits * NC) * (HD + 2);
-    const uint64_t rs = (uint64_t)NC * (HD + 2);
-    for (uint32_t i = tid; i < cols * HD; i += TH) {
-        const uint32_t col = i / HD, d = i % HD;
-        float mm = -INFINITY, ll = 0.0f, acc = 0.0f;
-        for (uint32_t w = 0; w < splits; w++) mm = fmaxf(mm, __ldcg(r0 + w * rs + NC * HD + col));
-#pragma unroll 8
-        for (uint32_t w = 0; w < splits; w++) {
-            const float f = ex2(__ldcg(r0 + w * rs + NC * HD + col) - mm);
-            ll = fmaf(__ldcg(r0 + w * rs + NC * HD + NC + col), f, ll);
-            acc = fmaf(__ldcg(r0 + w * rs + i), f, acc);
+    if (tid == 0) *counter = 0;
+    for (uint32_t i = i0 + tid; i < i1; i += THREADS) {
+        const uint32_t col = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (uint32_t c = 0; c < n_cl; c++) {
+            const float* r = rec0 + c * REC;
+            const float mc = __ldcg(r + stats + col), lc = __ldcg(r + stats + NC + col);
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(r + 4 * i));
+            const float up = fmaxf(mm, mc), f = up == mm ? 1.0f : ex2(mm - up), fc = ex2(mc - up);
+            mm = up;
+            ll = fmaf(lc, fc, ll * f);
+            acc.x = fmaf(x.x, fc, acc.x * f), acc.y = fmaf(x.y, fc, acc.y * f);
+            acc.z = fmaf(x.z, fc, acc.z * f), acc.w = fmaf(x.w, fc, acc.w * f);
         }
-        store1<DT>(const_cast<void*>(a.out.p), slot * a.out.row + (uint64_t)(h0 + col) * a.out.head + d, acc / ll);
+        store(col, d, acc, ll);
     }
 }
 
@@ -432,14 +557,42 @@ cudaError_t attend_dt(const Kv8AttendArgs& a, cudaStream_t st) {
         k_kv8_attend_simple<HD, DT><<<(uint32_t)((items + 3) / 4), 128, 0, st>>>(a);
         return cudaGetLastError();
     }
-    const uint32_t nc = kv8_single_cols(a.nh / a.kv.nkv);
-    const dim3 grid(a.rows.n_slots * a.kv.nkv * ((a.nh / a.kv.nkv + nc - 1) / nc), a.max_splits);
-    if (nc == 8) k_kv8_single<HD, DT, 1><<<grid, kDecWarps * 32, 0, st>>>(a);
-    else k_kv8_single<HD, DT, 2><<<grid, kDecWarps * 32, 0, st>>>(a);
-    return cudaGetLastError();
+    const bool wide = kv8_single_cols(a.group) == 16;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.kv.nkv * a.chunks, (a.max_splits + a.cluster - 1) / a.cluster * a.cluster, a.rows.n_slots);
+    cfg.blockDim = dim3(wide ? DecGeom<HD, DT, 2>::THREADS : DecGeom<HD, DT, 1>::THREADS);
+    cfg.dynamicSmemBytes = wide ? DecGeom<HD, DT, 2>::RING : DecGeom<HD, DT, 1>::RING;
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1;
+    attr.val.clusterDim.y = a.cluster;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return wide ? cudaLaunchKernelEx(&cfg, k_kv8_single<HD, DT, 2>, a) : cudaLaunchKernelEx(&cfg, k_kv8_single<HD, DT, 1>, a);
+}
+
+template <int HD, int DT>
+cudaError_t set_limits() {
+    cudaError_t e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 1>::RING);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 2>::RING);
+    return e;
 }
 
 }  // namespace
+
+// Per device, before the first launch there.
+cudaError_t kv8_attend_set_smem_limits() {
+    cudaError_t e = set_limits<64, HS_F32>();
+    if (e == cudaSuccess) e = set_limits<64, HS_F16>();
+    if (e == cudaSuccess) e = set_limits<64, HS_BF16>();
+    if (e == cudaSuccess) e = set_limits<128, HS_F32>();
+    if (e == cudaSuccess) e = set_limits<128, HS_F16>();
+    if (e == cudaSuccess) e = set_limits<128, HS_BF16>();
+    return e;
+}
 
 cudaError_t launch_kv8_attend(uint32_t hd, const Kv8AttendArgs& a, cudaStream_t st) {
     if (!a.rows.n_rows) return cudaSuccess;

@@ -93,32 +93,44 @@ cudaError_t launch_kv8_read(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows,
                             cudaStream_t st);
 
 // A single row's positions are split between CTAs by its own length and the
-// region's shape alone, so that its bits do not depend on the batch: 64 KB of
-// codes a split, and from about one CTA a KV head and SM (of a B200's 148) on
-// fewer, longer ones.
+// region's shape alone, so that its bits do not depend on the batch: in
+// eight (a cluster), but splits of at least 32 KB and at most 128 KB of codes
+// and no more than kv8_max_splits. Short splits finish a lone row sooner (2,048
+// positions, 14/2 heads of 64: 5.9 us in eight, 7.6 in four), long ones keep a
+// large batch's CTAs from spending their time on starting and joining (64
+// sequences of 8,192: 46 us with 128 KB, 58 with 64 KB).
 constexpr uint32_t kv8_max_splits(uint32_t nkv) {
-    return nkv <= 1 ? 148 : 148 / nkv < 16 ? 16 : 148 / nkv;
+    return nkv <= 2 ? 148 : 296 / nkv < 16 ? 16 : 296 / nkv;
 }
-__host__ __device__ constexpr uint32_t kv8_min_split(uint32_t hd) { return 32768 / hd; }
+__host__ __device__ constexpr uint32_t kv8_min_split(uint32_t hd) { return 16384 / hd; }
 __host__ __device__ inline uint32_t kv8_split_len(uint32_t n, uint32_t hd, uint32_t max_splits) {
-    const uint32_t len = ((n + max_splits - 1) / max_splits + 63) / 64 * 64, least = kv8_min_split(hd);
-    return len > least ? len : least;
+    const uint32_t least = kv8_min_split(hd), most = 4 * least;
+    uint32_t len = (n / 8 + 63) / 64 * 64;
+    len = len < least ? least : len > most ? most : len;
+    if (n <= len * max_splits) return len;
+    return ((n + max_splits - 1) / max_splits + 63) / 64 * 64;
 }
 // Query heads of one KV head that a CTA takes together.
 constexpr uint32_t kv8_single_cols(uint32_t group) { return group <= 8 ? 8 : 16; }
+
+// Floats of a cluster's record: outputs, and for each of 8 shares its columns' maxima and sums.
+__host__ __device__ constexpr uint32_t kv8_record(uint32_t hd, uint32_t cols) { return cols * (hd + 16); }
 
 struct Kv8AttendArgs {
     Kv8View kv;
     Kv8Rows rows;
     Kv8Mat q, out;
-    uint32_t nh = 0;
+    uint32_t nh = 0, group = 0, chunks = 0;  // query heads, per KV head, and CTAs of kv8_single_cols for these
     float scale = 1.0f;
-    // single rows: split records [slot][KV head][head chunk][split][cols x (head_dim + 2)]
-    // and, for each (slot, KV head, chunk), a counter that is zero between calls
+    // single rows: CTAs of `cluster` splits join in shared memory; where a
+    // region's rows can need more of them, their records [slot][KV head][head
+    // chunk][max_clusters][kv8_record] and, for each (slot, KV head, chunk),
+    // eight counters that are zero between calls
+    uint32_t max_splits = 0, cluster = 1, max_clusters = 0;
     float* part = nullptr;
     uint32_t* counters = nullptr;
-    uint32_t max_splits = 0;
 };
+cudaError_t kv8_attend_set_smem_limits();
 cudaError_t launch_kv8_attend(uint32_t hd, const Kv8AttendArgs& a, cudaStream_t st);
 
 #ifdef __CUDACC__
