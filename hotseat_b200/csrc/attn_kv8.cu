@@ -17,6 +17,7 @@
 #include "device.cuh"
 #include "kernels.h"
 #include "kv8.h"
+#include "tcgen05.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -34,48 +35,6 @@ __device__ __forceinline__ void store1(void* p, uint64_t e, float x) {
     if constexpr (DT == HS_F32) static_cast<float*>(p)[e] = x;
     else if constexpr (DT == HS_F16) static_cast<__half*>(p)[e] = __float2half_rn(x);
     else static_cast<__nv_bfloat16*>(p)[e] = __float2bfloat16_rn(x);
-}
-
-// One warp per (row, query head): the positions in turn, with the running
-// maximum and sum of the softmax.
-template <int HD, int DT>
-__global__ void __launch_bounds__(128) k_kv8_attend_simple(const Kv8AttendArgs a) {
-    constexpr uint32_t N = HD / 32;
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const uint64_t r = item / a.nh;
-    const uint32_t h = (uint32_t)(item - r * a.nh), kvh = h / (a.nh / a.kv.nkv);
-    if (r >= a.rows.n_rows || (a.rows.row_start && r >= a.rows.row_start[a.rows.n_slots])) return;
-    float q[N], o[N], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < N; i++) {
-        q[i] = load1<DT>(a.q.p, r * a.q.row + h * a.q.head + lane * N + i) * a.scale;
-        o[i] = 0.0f;
-    }
-    uint32_t slot, pos;
-    if (kv8_place(a.rows, a.kv.max_ctx, (uint32_t)r, &slot, &pos)) {
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
-        for (uint32_t p = 0; p <= pos; p++) {
-            const int8_t* kc = reinterpret_cast<const int8_t*>(base + a.kv.code_off(0, kvh, p)) + lane * N;
-            const int8_t* vc = reinterpret_cast<const int8_t*>(base + a.kv.code_off(1, kvh, p)) + lane * N;
-            const float ks = *reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, p >> a.kv.block_shift));
-            const float vs = *reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, p >> a.kv.block_shift));
-            float s = 0.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) s = fmaf(q[i], (float)kc[i], s);
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            s *= ks;
-            const float mn = fmaxf(m, s), c = expf(m - mn), w = expf(s - mn);
-            l = l * c + w;
-            m = mn;
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) o[i] = fmaf(w * vs, (float)vc[i], o[i] * c);
-        }
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < N; i++)
-        store1<DT>(const_cast<void*>(a.out.p), r * a.out.row + h * a.out.head + lane * N + i, l > 0.0f || isnan(l) ? o[i] / l : 0.0f);
 }
 
 // ------------------------------------------------------------- single rows
@@ -550,11 +509,432 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
     }
 }
 
+// ------------------------------------------------------------------- chunks
+
+// Rows of prompts and chunks of them, on the fifth-generation tensor cores.
+// A CTA takes 256 of the (row, head of the group) pairs of one (slot, KV
+// head) and walks the positions in tiles of 128:
+//
+//   warps 0-3, 4-7  one 128-row tile each, a thread a row: scores from TMEM,
+//                   softmax, weights back to TMEM over the scores they came
+//                   from, the tile's outputs from TMEM into f32 registers;
+//                   the first thread issues the tile's MMAs
+//   warps 8-11      codes from the cache to f16 tiles in shared memory: K as
+//                   it lies, V transposed
+//
+//   S = Q K^T    A = Q (shared), B = K (shared), 128 x 128
+//   O' = W V     A = W (TMEM),   B = V^T (shared), 128 x head_dim
+//
+// While one row tile's threads are at their softmax the other's products run.
+// O' is summed over one tile of positions only and then added in registers:
+// sums over thousands of positions stay f32 with rounding to nearest, and a
+// rise of the maximum costs no pass over TMEM.
+template <int HD, int DT>
+struct ChunkGeom {
+    static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
+    static constexpr uint32_t KT = 128, ROWS = 256, THREADS = 384;
+    static constexpr uint32_t SLAB = 128 * 128;            // 128 rows of 64 f16
+    static constexpr uint32_t Q_BYTES = HD / 64 * SLAB;    // one row tile, hi or lo
+    static constexpr uint32_t K_BYTES = HD / 64 * SLAB, V_BYTES = 2 * HD * 128;
+    static constexpr uint32_t NB = HD == 128 && QPAIR ? 1 : 2;  // K and V buffers
+    static constexpr uint32_t Q_AT = 0, K_AT = Q_AT + 2 * (QPAIR ? 2 : 1) * Q_BYTES, V_AT = K_AT + NB * K_BYTES;
+    static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: K [NB][128], V [NB][128]
+    static constexpr uint32_t BYTES = SC_AT + NB * 2 * KT * 4 + 1024;
+    static constexpr uint32_t S_COL = 0, O_COL = 256;       // TMEM columns: S of both tiles, O' of both
+    static constexpr bool HOLD = HD == 64;                  // scores stay in registers between maximum and weights
+};
+
+constexpr uint32_t kChunkLimit = 1u << 22;
+// Registers a thread of the row tiles' warps and of the code warps; the
+// launch's 168 a thread cover two of the first and one of the second.
+constexpr int kChunkRegsRow = 200, kChunkRegsCode = 104;
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_sync(uint32_t id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+
+template <int HD, int DT>
+__global__ void __launch_bounds__(384, 1) k_kv8_chunk(const Kv8AttendArgs a) {
+    using G = ChunkGeom<HD, DT>;
+    constexpr uint32_t KT = G::KT, NB = G::NB;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t kfull[NB], kempty[NB], vfull[NB], vempty[NB], s_done[2], o_done[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ float vtop[4], vratio[NB], vunit;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t group = a.group;
+
+    // the tile: slot, its rows' first pair, its last position. Tiles of slot i
+    // start at row_start[i] * group / 256 + i, room for all that it can have.
+    const uint32_t bt = gridDim.x / a.kv.nkv - 1 - blockIdx.x / a.kv.nkv, kvh = blockIdx.x % a.kv.nkv;  // long ones first
+    uint32_t lo = 0, hi = a.rows.n_slots;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if ((uint64_t)__ldg(a.rows.row_start + mid) * group / G::ROWS + mid <= bt)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    if (lo == 0) return;
+    const uint32_t slot = lo - 1, r0 = __ldg(a.rows.row_start + slot);
+    const uint32_t r1 = min(__ldg(a.rows.row_start + slot + 1), a.rows.n_rows), m = r1 > r0 ? r1 - r0 : 0;
+    const uint64_t f0 = (bt - ((uint64_t)r0 * group / G::ROWS + slot)) * G::ROWS, pairs = (uint64_t)m * group;
+    if (f0 >= pairs) return;
+    const uint32_t pos0 = __ldg(a.rows.pos + slot);
+    const uint32_t live = (uint32_t)min((uint64_t)G::ROWS, pairs - f0);  // pairs of this CTA
+    const uint32_t jlast = (uint32_t)((f0 + live - 1) / group);          // its last row
+    if (pos0 == kPosNone || (uint64_t)pos0 + (uint32_t)(f0 / group) >= a.kv.max_ctx) {  // nothing to see
+        if (pos0 != kPosNone && tid == 0) atomicOr(a.rows.err, ERR_POS);
+        for (uint32_t i = tid; i < live * HD; i += G::THREADS) {
+            const uint64_t f = f0 + i / HD;
+            store1<DT>(const_cast<void*>(a.out.p), (r0 + f / group) * a.out.row + (kvh * group + f % group) * a.out.head + i % HD, 0.0f);
+        }
+        return;
+    }
+    const uint64_t plast = (uint64_t)pos0 + jlast;
+    if (plast >= a.kv.max_ctx && tid == 0) atomicOr(a.rows.err, ERR_POS);
+    const uint32_t end = (uint32_t)min(plast + 1, (uint64_t)a.kv.max_ctx);  // positions seen: [0, end)
+    const uint32_t tiles = (end + KT - 1) / KT;
+    const uint32_t users = live > 128 ? 2 : 1;  // row tiles at work
+
+    if (tid == 0) {
+        for (uint32_t i = 0; i < NB; i++) {
+            mbar_init(&kfull[i], 128);
+            mbar_init(&vfull[i], 128);
+            mbar_init(&kempty[i], users);
+            mbar_init(&vempty[i], users);
+        }
+        for (uint32_t i = 0; i < 2; i++) {
+            mbar_init(&s_done[i], 1);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init_fence();
+    }
+    if (warp == 0) {
+        tc5::alloc(&tmem_slot, 512);
+        tc5::relinquish();
+    }
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    const uint32_t tmem = tmem_slot;
+    float* sc = reinterpret_cast<float*>(smem + G::SC_AT);  // [NB][K 128 | V 128]
+    // A wait that runs out marks the call and no longer waits: every thread
+    // still passes every barrier, and the CTA ends.
+    bool dead = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait_bounded(bar, parity, kChunkLimit)) {
+            dead = true;
+            atomicOr(a.rows.err, ERR_TIMEOUT);
+        }
+    };
+
+    if (warp >= 8) {
+        // ---------------------------------------------------- codes to f16
+        tc5::setmaxnreg_dec<kChunkRegsCode>();
+        const uint32_t th = tid - 256;
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
+        const uint8_t* kp = base + a.kv.code_off(0, kvh, 0);
+        const uint8_t* vp = base + a.kv.code_off(1, kvh, 0);
+        const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, 0));
+        const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, 0));
+        const uint64_t ps = a.kv.pos_stride;
+        // K: a thread's 16 codes of a row, eight passes over the rows
+        constexpr uint32_t CPR = HD / 16, RPP = 128 / CPR, KP = KT / RPP;
+        const uint32_t kc = th % CPR, kr = th / CPR;
+        // V: eight positions (one 16-byte piece of a transposed row) by HD / 8 of d
+        constexpr uint32_t DW = HD / 32;  // words of a V row that a thread takes
+        const uint32_t vg = (th / 64) * 8 + th % 8, vd = ((th % 64) / 8) * (HD / 8);
+        uint4 kw[KP];
+        uint32_t vw[8][DW];
+        float ks, vs;
+        auto load_k = [&](uint32_t t) {
+#pragma unroll
+            for (uint32_t i = 0; i < KP; i++)
+                kw[i] = __ldg(reinterpret_cast<const uint4*>(kp + min(t * KT + kr + i * RPP, end - 1) * ps + 16 * kc));
+            ks = __ldg(ksp + (min(t * KT + th, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride);
+        };
+        auto load_v = [&](uint32_t t) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint8_t* p = vp + min(t * KT + 8 * vg + i, end - 1) * ps + vd;
+                if constexpr (HD == 64) {
+                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+                    vw[i][0] = w.x, vw[i][1] = w.y;
+                } else {
+                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+                    vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+                }
+            }
+            vs = t * KT + th < end ? __ldg(vsp + (min(t * KT + th, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride) : 0.0f;
+        };
+        float vmax = 0.0f, vfit = 0.0f;
+        load_k(0);
+        load_v(0);
+        for (uint32_t t = 0; t < tiles; t++) {
+            const uint32_t b = t % NB, use = t / NB;
+            if (use > 0) wait(&kempty[b], (use - 1) & 1);
+            uint8_t* kt = smem + G::K_AT + b * G::K_BYTES;
+#pragma unroll
+            for (uint32_t i = 0; i < KP; i++) {
+                const uint32_t r = kr + i * RPP;
+                const uint4 w = kw[i];
+                // codes 0, 2, 1, 3 of every four, as q's elements lie
+                const uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
+                const uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
+                const uint32_t c = 2 * kc, flip = kc / 4 & 1;  // the slabs' lanes write different banks
+                uint8_t* row = kt + c / 8 * G::SLAB + r * 128;
+                uint8_t *px = row + ((c % 8) ^ (r & 7)) * 16, *py = row + ((c % 8 + 1) ^ (r & 7)) * 16;
+                *reinterpret_cast<uint4*>(flip ? py : px) = flip ? y : x;
+                *reinterpret_cast<uint4*>(flip ? px : py) = flip ? x : y;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&kfull[b]);
+            const float ks_now = ks;
+            if (t + 1 < tiles) load_k(t + 1);
+
+            // V's scales under a power of two at or above the largest so far
+            float top = vs;
+#pragma unroll
+            for (uint32_t d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (use > 0) wait(&vempty[b], (use - 1) & 1);
+            if (lane == 0) vtop[warp - 8] = top;
+            bar_sync(3);
+            top = fmaxf(fmaxf(vtop[0], vtop[1]), fmaxf(vtop[2], vtop[3]));
+            float ratio = 1.0f;
+            if (top > vmax) {
+                const uint32_t e = min((__float_as_uint(top) >> 23) + 1, 254u);
+                const float fit = __uint_as_float(min(264u - e, 254u) << 23);
+                ratio = vfit > 0.0f ? fit / vfit : 1.0f;
+                vfit = fit;
+                vmax = __uint_as_float(e << 23);
+            }
+            // both tiles' scales go with V: they are read until the weights are written
+            sc[b * 2 * KT + th] = ks_now;
+            sc[b * 2 * KT + KT + th] = vs * vfit;
+            if (th == 0) {
+                vratio[b] = ratio;
+                if (t + 1 == tiles) vunit = vfit > 0.0f ? 1.0f / vfit : 0.0f;
+            }
+            uint8_t* vt = smem + G::V_AT + b * G::V_BYTES + (vg / 8) * (HD * 128);
+#pragma unroll
+            for (uint32_t i = 0; i < DW; i++) {
+                uint32_t f[4][4];  // d, d + 1, d + 2, d + 3 by position pairs
+#pragma unroll
+                for (uint32_t p = 0; p < 4; p++) {
+                    const uint32_t w0 = vw[2 * p][i], w1 = vw[2 * p + 1][i];
+                    const uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w0, w1, 0x7632);
+                    f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x), f[2][p] = even_bytes(y), f[3][p] = odd_bytes(y);
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    const uint32_t d = vd + 4 * i + e;
+                    *reinterpret_cast<uint4*>(vt + d * 128 + ((vg % 8) ^ (d & 7)) * 16) = make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]);
+                }
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&vfull[b]);
+            if (t + 1 < tiles) load_v(t + 1);
+            bar_sync(3);  // vtop is free
+        }
+    } else {
+        // ---------------------------------------------------- one row tile
+        tc5::setmaxnreg_inc<kChunkRegsRow>();
+        const uint32_t w = warp / 4, th = tid % 128, row = w * 128 + th;
+        if (w < users) {
+            const bool on = row < live;
+            const uint64_t f = f0 + row;
+            const uint32_t j = (uint32_t)(f / group), h = kvh * group + (uint32_t)(f - (uint64_t)j * group);
+            const uint64_t p = (uint64_t)pos0 + j;
+            const int lim = on && p < a.kv.max_ctx ? (int)p : -1;  // the last position this row sees
+            uint8_t* qt = smem + G::Q_AT + w * G::Q_BYTES;
+            float cf;
+            {
+                // q to f16 rows of 64, elements 0, 2, 1, 3 of every four as K's codes lie
+                const uint64_t at = (r0 + (uint64_t)j) * a.q.row + (uint64_t)h * a.q.head;
+                float top = 0.0f;
+                if (on)
+                    for (uint32_t d = 0; d < HD; d++) top = fmaxf(top, fabsf(load1<DT>(a.q.p, at + d)));
+                float inv;
+                const float fit = fit_f16(top, &inv);
+                cf = (a.scale * kLog2e) * inv;
+#pragma unroll 4
+                for (uint32_t c = 0; c < HD / 8; c++) {
+                    float x[8];
+                    uint32_t hi4[4], lo4[4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) x[e] = on ? load1<DT>(a.q.p, at + 8 * c + e) * fit : 0.0f;
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; e++) {
+                        pair16(x[4 * e], x[4 * e + 2], &hi4[2 * e], &lo4[2 * e]);
+                        pair16(x[4 * e + 1], x[4 * e + 3], &hi4[2 * e + 1], &lo4[2 * e + 1]);
+                    }
+                    uint8_t* to = qt + c / 8 * G::SLAB + th * 128 + ((c % 8) ^ (th & 7)) * 16;
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+                    if constexpr (G::QPAIR) *reinterpret_cast<uint4*>(to + 2 * G::Q_BYTES) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            bar_sync(1 + w);
+
+            const uint32_t scol = tmem + G::S_COL + w * KT, ocol = tmem + G::O_COL + w * HD;
+            const uint32_t lanes = (warp % 4 * 32) << 16;
+            auto issue_s = [&](uint32_t t) {
+                const uint32_t b = t % NB;
+                wait(&kfull[b], t / NB & 1);
+                tc5::fence_after();
+                const uint32_t kb = smem_u32(smem + G::K_AT + b * G::K_BYTES), qb = smem_u32(qt);
+#pragma unroll
+                for (uint32_t k = 0; k < HD / 16; k++) {
+                    const uint64_t kd = tc5::sw128_desc(kb + k / 4 * G::SLAB) + 2 * (k % 4);
+                    const uint64_t qd = tc5::sw128_desc(qb + k / 4 * G::SLAB) + 2 * (k % 4);
+                    if constexpr (G::QPAIR) {
+                        const uint64_t ld = tc5::sw128_desc(qb + 2 * G::Q_BYTES + k / 4 * G::SLAB) + 2 * (k % 4);
+                        tc5::mma_ss(scol, ld, kd, tc5::idesc_f16(128, KT), k > 0);
+                        tc5::mma_ss(scol, qd, kd, tc5::idesc_f16(128, KT), true);
+                    } else {
+                        tc5::mma_ss(scol, qd, kd, tc5::idesc_f16(128, KT), k > 0);
+                    }
+                }
+                tc5::commit(&s_done[w]);
+                tc5::commit(&kempty[b]);
+            };
+            auto issue_o = [&](uint32_t t) {
+                const uint32_t b = t % NB;
+                wait(&vfull[b], t / NB & 1);
+                tc5::fence_after();
+                const uint32_t vb = smem_u32(smem + G::V_AT + b * G::V_BYTES);
+#pragma unroll
+                for (uint32_t k = 0; k < KT / 16; k++) {
+                    const uint64_t vd = tc5::sw128_desc(vb + k / 4 * (HD * 128)) + 2 * (k % 4);
+                    const uint32_t wc = scol + k / 2 * 32 + k % 2 * 8;
+                    if constexpr (G::WPAIR) {
+                        tc5::mma_ts(ocol, wc + 16, vd, tc5::idesc_f16(128, HD), k > 0);
+                        tc5::mma_ts(ocol, wc, vd, tc5::idesc_f16(128, HD), true);
+                    } else {
+                        tc5::mma_ts(ocol, wc, vd, tc5::idesc_f16(128, HD), k > 0);
+                    }
+                }
+                tc5::commit(&o_done[w]);
+                tc5::commit(&vempty[b]);
+            };
+            if (th == 0) issue_s(0);
+
+            float o[HD], mx = -INFINITY, l = 0.0f, alpha = 1.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < HD; i++) o[i] = 0.0f;
+            auto add_o = [&](uint32_t t) {  // the outputs of tile t, once they are there
+                wait(&o_done[w], t & 1);
+                tc5::fence_after();
+#pragma unroll
+                for (uint32_t c = 0; c < HD / 32; c++) {
+                    float x[32];
+                    tc5::ld32(ocol + lanes + 32 * c, x);
+                    tc5::wait_ld();
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i++) o[32 * c + i] = fmaf(o[32 * c + i], alpha, x[i]);
+                }
+            };
+            for (uint32_t t = 0; t < tiles; t++) {
+                const uint32_t b = t % NB;
+                const float* ks = sc + b * 2 * KT;
+                const int left = lim - (int)(t * KT);  // columns 0..left are seen
+                const bool full = __all_sync(0xffffffffu, left >= (int)KT - 1);
+                wait(&vfull[b], t / NB & 1);
+                wait(&s_done[w], t & 1);
+                tc5::fence_after();
+                float s[G::HOLD ? KT : 32], top = -INFINITY;
+                auto scores = [&](uint32_t c, float* x) {  // columns 32 c.. under K's scales, unseen ones -inf
+                    tc5::ld32(scol + lanes + 32 * c, x);
+                    tc5::wait_ld();
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(ks + 32 * c + i);
+                        x[i] *= k4.x, x[i + 1] *= k4.y, x[i + 2] *= k4.z, x[i + 3] *= k4.w;
+                    }
+                    if (!full) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 32; i++)
+                            if ((int)(32 * c + i) > left) x[i] = -INFINITY;
+                    }
+                };
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    float* x = s + (G::HOLD ? 32 * c : 0);
+                    scores(c, x);
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i++) top = fmaxf(top, x[i]);
+                }
+                if (t > 0) add_o(t - 1);
+                alpha = 1.0f;
+                if ((top - mx) * cf > kSlack) {
+                    alpha = ex2((mx - top) * cf);
+                    mx = top;
+                    l *= alpha;
+                }
+                const float off = mx == -INFINITY ? 0.0f : -mx * cf;
+                alpha *= vratio[b];
+                const float* vs = ks + KT;
+                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    float* x = s + (G::HOLD ? 32 * c : 0);
+                    if constexpr (!G::HOLD) scores(c, x);
+                    uint32_t wh[16], wl[16];
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; i += 4) {
+                        const float4 v4 = *reinterpret_cast<const float4*>(vs + 32 * c + i);
+                        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+                        float y[4];
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; e++) {
+                            const bool out = !full && (int)(32 * c + i + e) > left;
+                            const float pr = out ? 0.0f : ex2(fmaf(x[i + e], cf, off));
+                            l4[e] += pr;
+                            y[e] = out ? 0.0f : pr * v[e];  // a scale of NaN does not reach rows before it
+                        }
+                        pair16(y[0], y[1], &wh[i / 2], &wl[i / 2]);
+                        pair16(y[2], y[3], &wh[i / 2 + 1], &wl[i / 2 + 1]);
+                    }
+                    tc5::st16(scol + lanes + 32 * c, wh);
+                    if constexpr (G::WPAIR) tc5::st16(scol + lanes + 32 * c + 16, wl);
+                }
+                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                tc5::wait_st();
+                tc5::fence_before();
+                bar_sync(1 + w);
+                if (th == 0) {
+                    tc5::fence_after();
+                    issue_o(t);
+                    if (t + 1 < tiles) issue_s(t + 1);
+                }
+                __syncwarp();
+            }
+            add_o(tiles - 1);
+            if (on) {
+                const float unit = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
+                const uint64_t at = (r0 + (uint64_t)j) * a.out.row + (uint64_t)h * a.out.head;
+#pragma unroll
+                for (uint32_t i = 0; i < HD; i++) store1<DT>(const_cast<void*>(a.out.p), at + i, lim >= 0 ? o[i] * unit : 0.0f);
+            }
+        }
+    }
+    tc5::fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc5::fence_after();
+        tc5::dealloc(tmem, 512);
+    }
+}
+
 template <int HD, int DT>
 cudaError_t attend_dt(const Kv8AttendArgs& a, cudaStream_t st) {
     if (a.rows.row_start) {
-        const uint64_t items = (uint64_t)a.rows.n_rows * a.nh;
-        k_kv8_attend_simple<HD, DT><<<(uint32_t)((items + 3) / 4), 128, 0, st>>>(a);
+        using G = ChunkGeom<HD, DT>;
+        const uint64_t tiles = (uint64_t)a.rows.n_rows * a.group / G::ROWS + a.rows.n_slots;
+        k_kv8_chunk<HD, DT><<<(uint32_t)(tiles * a.kv.nkv), G::THREADS, G::BYTES, st>>>(a);
         return cudaGetLastError();
     }
     const bool wide = kv8_single_cols(a.group) == 16;
@@ -578,6 +958,12 @@ cudaError_t set_limits() {
     cudaError_t e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 1>::RING);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 2>::RING);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(k_kv8_chunk<HD, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkGeom<HD, DT>::BYTES);
+    // the chunk kernel deals the registers of its launch out anew: all of them must be there
+    cudaFuncAttributes at{};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, k_kv8_chunk<HD, DT>);
+    if (e == cudaSuccess && at.numRegs * 3 < kChunkRegsRow * 2 + kChunkRegsCode) e = cudaErrorInvalidConfiguration;
     return e;
 }
 

@@ -214,6 +214,7 @@ int hs_kv8_set_check(hs_kv8_set* s, void* stream) {
     HS_CUDA_TRY(cudaMemcpyAsync(s->err_h, s->err, 4, cudaMemcpyDeviceToHost, st));
     HS_CUDA_TRY(cudaMemsetAsync(s->err, 0, 4, st));
     HS_CUDA_TRY(cudaStreamSynchronize(st));
+    if (*s->err_h & ERR_TIMEOUT) return fail(HS_E_CUDA, "attention reported a bounded-wait timeout");
     if (*s->err_h & ERR_POS) return fail(HS_E_ARG, "position past max_ctx");
     return HS_OK;
 }
