@@ -37,6 +37,46 @@ __device__ __forceinline__ void store1(void* p, uint64_t e, float x) {
     else static_cast<__nv_bfloat16*>(p)[e] = __float2bfloat16_rn(x);
 }
 
+// Four consecutive elements; `vec`: at once, where base and strides allow it.
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, uint64_t e, bool vec, float* x) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = load1<DT>(p, e + i);
+    } else if constexpr (DT == HS_F32) {
+        const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + e);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + e);
+        const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if constexpr (DT == HS_F16) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                x[2 * i] = f.x, x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store4(void* p, uint64_t e, bool vec, float4 v) {
+    if (!vec) {
+        store1<DT>(p, e, v.x), store1<DT>(p, e + 1, v.y), store1<DT>(p, e + 2, v.z), store1<DT>(p, e + 3, v.w);
+    } else if constexpr (DT == HS_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + e) = v;
+    } else if constexpr (DT == HS_F16) {
+        const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + e) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + e) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
 // ------------------------------------------------------------- single rows
 
 __device__ __forceinline__ float ex2(float x) {
@@ -426,10 +466,7 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
     auto store = [&](uint32_t col, uint32_t d, float4 acc, float ll) {
         const uint64_t at = slot * a.out.row + (uint64_t)(h0 + col) * a.out.head + d;
         const float inv = __frcp_rn(ll);
-        store1<DT>(const_cast<void*>(a.out.p), at, acc.x * inv);
-        store1<DT>(const_cast<void*>(a.out.p), at + 1, acc.y * inv);
-        store1<DT>(const_cast<void*>(a.out.p), at + 2, acc.z * inv);
-        store1<DT>(const_cast<void*>(a.out.p), at + 3, acc.w * inv);
+        store4<DT>(const_cast<void*>(a.out.p), at, a.out_vec, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     };
     if (splits == 1) {
         __syncthreads();
@@ -519,51 +556,79 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 //                   softmax, weights back to TMEM over the scores they came
 //                   from, the tile's outputs from TMEM into f32 registers;
 //                   the first thread issues the tile's MMAs
-//   warps 8-11      codes from the cache to f16 tiles in shared memory: K as
-//                   it lies, V transposed
+//   warps 8-15      codes from the cache to f16 tiles in shared memory, 16
+//                   positions a warp: K as it lies, V transposed. A warp loads
+//                   a tile's codes into registers as it writes the one
+//                   before, and waits for no other warp.
 //
 //   S = Q K^T    A = Q (shared), B = K (shared), 128 x 128
 //   O' = W V     A = W (TMEM),   B = V^T (shared), 128 x head_dim
 //
 // While one row tile's threads are at their softmax the other's products run.
-// O' is summed over one tile of positions only and then added in registers:
-// sums over thousands of positions stay f32 with rounding to nearest, and a
-// rise of the maximum costs no pass over TMEM.
 template <int HD, int DT>
 struct ChunkGeom {
     static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
-    static constexpr uint32_t KT = 128, ROWS = 256, THREADS = 384;
+    static constexpr uint32_t KT = 128, ROWS = 256, THREADS = 512;
     static constexpr uint32_t SLAB = 128 * 128;            // 128 rows of 64 f16
     static constexpr uint32_t Q_BYTES = HD / 64 * SLAB;    // one row tile, hi or lo
     static constexpr uint32_t K_BYTES = HD / 64 * SLAB, V_BYTES = 2 * HD * 128;
     static constexpr uint32_t NB = HD == 128 && QPAIR ? 1 : 2;  // K and V buffers
     static constexpr uint32_t Q_AT = 0, K_AT = Q_AT + 2 * (QPAIR ? 2 : 1) * Q_BYTES, V_AT = K_AT + NB * K_BYTES;
     static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: K [NB][128], V [NB][128]
-    static constexpr uint32_t BYTES = SC_AT + NB * 2 * KT * 4 + 1024;
+    static constexpr uint32_t BYTES = SC_AT + (DT == HS_BF16 ? 0 : NB * 2 * KT * 4) + 1024;
     static constexpr uint32_t S_COL = 0, O_COL = 256;       // TMEM columns: S of both tiles, O' of both
-    static constexpr bool HOLD = HD == 64;                  // scores stay in registers between maximum and weights
+    // bf16 rows take the scales with the codes (K and V rounded to f16, 2^-11 a
+    // value against the 2^-8 of their own type): 2.5 operations a score less.
+    // The others keep them outside, on scores and weights.
+    static constexpr bool FOLD = DT == HS_BF16;
+    // 2^VEXP is at least the largest V scale (FOLD: of the codes' f16 rows) and
+    // 2^PEXP what a weight of 1 is stored as
+    static constexpr uint32_t VEXP = FOLD ? 8 : 10;
+    static constexpr float PEXP = FOLD ? 8.0f : 0.0f;
 };
 
 constexpr uint32_t kChunkLimit = 1u << 22;
-// Registers a thread of the row tiles' warps and of the code warps; the
-// launch's 168 a thread cover two of the first and one of the second.
-constexpr int kChunkRegsRow = 200, kChunkRegsCode = 104;
+
+// Two f32 at once (each rounded on its own).
+__device__ __forceinline__ void mul2(float* x, float a, float b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(a, b)));
+    unpack2(r, x, x + 1);
+}
+__device__ __forceinline__ void fma2(float* x, float a, float b) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(a, a)), "l"(pack2(b, b)));
+    unpack2(r, x, x + 1);
+}
+__device__ __forceinline__ void add2(float* x, const float* y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(y[0], y[1])));
+    unpack2(r, x, x + 1);
+}
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void bar_sync(uint32_t id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+template <uint32_t N = 128>
+__device__ __forceinline__ void bar_sync(uint32_t id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
 
 template <int HD, int DT>
-__global__ void __launch_bounds__(384, 1) k_kv8_chunk(const Kv8AttendArgs a) {
+__global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
     using G = ChunkGeom<HD, DT>;
     constexpr uint32_t KT = G::KT, NB = G::NB;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t kfull[NB], kempty[NB], vfull[NB], vempty[NB], s_done[2], o_done[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ float vtop[4], vratio[NB], vunit;
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ float ktop[16], vtop[16], row_cf[G::ROWS];
+    __shared__ uint64_t row_q[G::ROWS], row_out[G::ROWS];  // element offsets of the tile's rows
+    // the warp's number as a value that is the same for its lanes
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t group = a.group;
 
     // the tile: slot, its rows' first pair, its last position. Tiles of slot i
@@ -601,8 +666,8 @@ __global__ void __launch_bounds__(384, 1) k_kv8_chunk(const Kv8AttendArgs a) {
 
     if (tid == 0) {
         for (uint32_t i = 0; i < NB; i++) {
-            mbar_init(&kfull[i], 128);
-            mbar_init(&vfull[i], 128);
+            mbar_init(&kfull[i], 8);  // a warp's arrival each
+            mbar_init(&vfull[i], 8);
             mbar_init(&kempty[i], users);
             mbar_init(&vempty[i], users);
         }
@@ -616,10 +681,37 @@ __global__ void __launch_bounds__(384, 1) k_kv8_chunk(const Kv8AttendArgs a) {
         tc5::alloc(&tmem_slot, 512);
         tc5::relinquish();
     }
+    // the largest scales that this CTA will meet, and powers of two to put them under
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
+    const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, 0));
+    const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, 0));
+    {
+        float kt = 0.0f, vt = 0.0f;
+        for (uint32_t i = tid; i <= (end - 1) >> a.kv.block_shift; i += G::THREADS) {
+            if constexpr (G::FOLD) kt = fmaxf(kt, __ldg(ksp + i * a.kv.sblk_stride));
+            vt = fmaxf(vt, __ldg(vsp + i * a.kv.sblk_stride));
+        }
+#pragma unroll
+        for (uint32_t d = 16; d > 0; d >>= 1) {
+            if constexpr (G::FOLD) kt = fmaxf(kt, __shfl_xor_sync(0xffffffffu, kt, d));
+            vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
+        }
+        if (lane == 0) ktop[warp] = kt, vtop[warp] = vt;
+    }
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
     const uint32_t tmem = tmem_slot;
+    // 2^exp over the power of two above the largest of them (1 if they are all 0), and its inverse
+    auto fit_under = [](const float* tops, uint32_t exp, float* inverse) {
+        float top = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++) top = fmaxf(top, tops[i]);
+        const uint32_t e = top > 0.0f ? min((__float_as_uint(top) >> 23) + 1, 253u) : 127u + exp;
+        const uint32_t bits = min(254u + exp - e, 253u);
+        *inverse = __uint_as_float((254u - bits) << 23);
+        return __uint_as_float(bits << 23);
+    };
     float* sc = reinterpret_cast<float*>(smem + G::SC_AT);  // [NB][K 128 | V 128]
     // A wait that runs out marks the call and no longer waits: every thread
     // still passes every barrier, and the CTA ends.
@@ -633,291 +725,384 @@ __global__ void __launch_bounds__(384, 1) k_kv8_chunk(const Kv8AttendArgs a) {
 
     if (warp >= 8) {
         // ---------------------------------------------------- codes to f16
-        tc5::setmaxnreg_dec<kChunkRegsCode>();
-        const uint32_t th = tid - 256;
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
-        const uint8_t* kp = base + a.kv.code_off(0, kvh, 0);
-        const uint8_t* vp = base + a.kv.code_off(1, kvh, 0);
-        const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, 0));
-        const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, 0));
+        const uint32_t cw = warp - 8;  // this warp's positions of a tile: 16 cw .. 16 cw + 15
         const uint64_t ps = a.kv.pos_stride;
-        // K: a thread's 16 codes of a row, eight passes over the rows
-        constexpr uint32_t CPR = HD / 16, RPP = 128 / CPR, KP = KT / RPP;
-        const uint32_t kc = th % CPR, kr = th / CPR;
-        // V: eight positions (one 16-byte piece of a transposed row) by HD / 8 of d
-        constexpr uint32_t DW = HD / 32;  // words of a V row that a thread takes
-        const uint32_t vg = (th / 64) * 8 + th % 8, vd = ((th % 64) / 8) * (HD / 8);
+        // K: a lane takes 16 codes of rows kr, kr + RPP, ...
+        constexpr uint32_t CPR = HD / 16, RPP = 32 / CPR, KP = 16 / RPP;
+        const uint32_t kc = lane % CPR, kr = lane / CPR;
+        float unit;
+        const float vfit = fit_under(vtop, G::VEXP, &unit);
+        const float kfit = G::FOLD ? fit_under(ktop, 7, &unit) : 1.0f;
+        // V: four codes of each of eight positions (a 16-byte piece of a
+        // transposed row), of position group vg, then vg + 1 where HD = 128.
+        // Element d = 4 dw + e goes to row e * HD / 4 + dw, so that the lanes'
+        // pieces fall into different banks; the outputs' columns follow.
+        constexpr uint32_t DW = HD / 4, VP = HD / 64;
+        const uint32_t dw = lane % DW, vg = 2 * cw + lane / DW;
+        const uint8_t* kp = base + a.kv.code_off(0, kvh, 0) + 16 * kc;
+        const uint8_t* vp = base + a.kv.code_off(1, kvh, 0) + 4 * dw;
         uint4 kw[KP];
-        uint32_t vw[8][DW];
+        uint32_t vw[VP][8];
         float ks, vs;
         auto load_k = [&](uint32_t t) {
+            const uint32_t p0 = t * KT + 16 * cw + kr;
+            if ((t + 1) * KT <= end) {
+                const uint8_t* q = kp + p0 * ps;
 #pragma unroll
-            for (uint32_t i = 0; i < KP; i++)
-                kw[i] = __ldg(reinterpret_cast<const uint4*>(kp + min(t * KT + kr + i * RPP, end - 1) * ps + 16 * kc));
-            ks = __ldg(ksp + (min(t * KT + th, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride);
+                for (uint32_t i = 0; i < KP; i++, q += RPP * ps) kw[i] = __ldg(reinterpret_cast<const uint4*>(q));
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < KP; i++)
+                    kw[i] = __ldg(reinterpret_cast<const uint4*>(kp + min(p0 + i * RPP, end - 1) * ps));
+            }
         };
         auto load_v = [&](uint32_t t) {
+            const uint32_t p0 = t * KT + 8 * vg;
+            if ((t + 1) * KT <= end) {
+                const uint8_t* q = vp + p0 * ps;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const uint8_t* p = vp + min(t * KT + 8 * vg + i, end - 1) * ps + vd;
-                if constexpr (HD == 64) {
-                    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
-                    vw[i][0] = w.x, vw[i][1] = w.y;
-                } else {
-                    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
-                    vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
-                }
+                for (uint32_t i = 0; i < VP * 8; i++, q += ps) vw[i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(q));
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < VP * 8; i++)
+                    vw[i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(vp + min(p0 + i, end - 1) * ps));
             }
-            vs = t * KT + th < end ? __ldg(vsp + (min(t * KT + th, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride) : 0.0f;
         };
-        float vmax = 0.0f, vfit = 0.0f;
+        auto load_s = [&](uint32_t t) {  // position 16 cw + lane % 16; behind the end: 0
+            const uint32_t p = t * KT + 16 * cw + lane % 16;
+            const float* at = ksp + (uint64_t)(min(p, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride;
+            ks = p < end ? __ldg(at) * kfit : 0.0f;
+            vs = p < end ? __ldg(at + a.kv.splane / 4) * vfit : 0.0f;
+        };
+        auto times = [](uint32_t x, uint32_t h) {
+            const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&h));
+            return *reinterpret_cast<const uint32_t*>(&y);
+        };
+        // places in the tiles of buffer 0: of a chunk's first half (the second
+        // lies beside it), of the pieces' row dw (the others DW rows on)
+        const uint32_t to_k = smem_u32(smem + G::K_AT) + kc / 4 * G::SLAB + (16 * cw + kr) * 128 + ((2 * kc % 8) ^ (kr & 7)) * 16;
+        const uint32_t to_v = smem_u32(smem + G::V_AT) + vg / 8 * (HD * 128) + dw * 128 + ((vg % 8) ^ (dw & 7)) * 16;
+        load_s(0);
         load_k(0);
         load_v(0);
         for (uint32_t t = 0; t < tiles; t++) {
             const uint32_t b = t % NB, use = t / NB;
+            uint32_t kh = 0, vh = 0;  // FOLD: position lane % 16's scale twice; positions 2 i, 2 i + 1 of lane i's
+            if constexpr (G::FOLD) {
+                // A NaN in either scale goes to the scores, where only the rows
+                // that see the position take it; V's row is then zeros.
+                const bool bad = isnan(vs);
+                const __half2 k2 = __float2half2_rn(bad ? vs : ks);
+                kh = *reinterpret_cast<const uint32_t*>(&k2);
+                const uint32_t v1 = __half_as_ushort(__float2half_rn(bad ? 0.0f : vs));
+                const uint32_t v0 = __shfl_sync(0xffffffffu, v1, 2 * lane), v2 = __shfl_sync(0xffffffffu, v1, 2 * lane + 1);
+                vh = v0 | v2 << 16;
+            }
+            const float ks_now = ks, vs_now = vs;
+            if (t + 1 < tiles) load_s(t + 1);
             if (use > 0) wait(&kempty[b], (use - 1) & 1);
-            uint8_t* kt = smem + G::K_AT + b * G::K_BYTES;
 #pragma unroll
             for (uint32_t i = 0; i < KP; i++) {
-                const uint32_t r = kr + i * RPP;
                 const uint4 w = kw[i];
                 // codes 0, 2, 1, 3 of every four, as q's elements lie
-                const uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
-                const uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
-                const uint32_t c = 2 * kc, flip = kc / 4 & 1;  // the slabs' lanes write different banks
-                uint8_t* row = kt + c / 8 * G::SLAB + r * 128;
-                uint8_t *px = row + ((c % 8) ^ (r & 7)) * 16, *py = row + ((c % 8 + 1) ^ (r & 7)) * 16;
-                *reinterpret_cast<uint4*>(flip ? py : px) = flip ? y : x;
-                *reinterpret_cast<uint4*>(flip ? px : py) = flip ? x : y;
+                uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
+                uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
+                if constexpr (G::FOLD) {
+                    const uint32_t h = __shfl_sync(0xffffffffu, kh, kr + i * RPP);
+                    x = make_uint4(times(x.x, h), times(x.y, h), times(x.z, h), times(x.w, h));
+                    y = make_uint4(times(y.x, h), times(y.y, h), times(y.z, h), times(y.w, h));
+                }
+                // rows RPP apart: their places' swizzle is the same where RPP is 8, else it flips bit 2
+                const uint32_t row = b * G::K_BYTES + i * RPP * 128, flip = RPP == 4 && (i & 1) ? 64 : 0;
+                sts128((to_k ^ flip) + row, x);
+                sts128((to_k ^ flip ^ 16) + row, y);
             }
             fence_proxy_async_smem();
-            mbar_arrive(&kfull[b]);
-            const float ks_now = ks;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kfull[b]);
             if (t + 1 < tiles) load_k(t + 1);
 
-            // V's scales under a power of two at or above the largest so far
-            float top = vs;
-#pragma unroll
-            for (uint32_t d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (use > 0) wait(&vempty[b], (use - 1) & 1);
-            if (lane == 0) vtop[warp - 8] = top;
-            bar_sync(3);
-            top = fmaxf(fmaxf(vtop[0], vtop[1]), fmaxf(vtop[2], vtop[3]));
-            float ratio = 1.0f;
-            if (top > vmax) {
-                const uint32_t e = min((__float_as_uint(top) >> 23) + 1, 254u);
-                const float fit = __uint_as_float(min(264u - e, 254u) << 23);
-                ratio = vfit > 0.0f ? fit / vfit : 1.0f;
-                vfit = fit;
-                vmax = __uint_as_float(e << 23);
-            }
-            // both tiles' scales go with V: they are read until the weights are written
-            sc[b * 2 * KT + th] = ks_now;
-            sc[b * 2 * KT + KT + th] = vs * vfit;
-            if (th == 0) {
-                vratio[b] = ratio;
-                if (t + 1 == tiles) vunit = vfit > 0.0f ? 1.0f / vfit : 0.0f;
-            }
-            uint8_t* vt = smem + G::V_AT + b * G::V_BYTES + (vg / 8) * (HD * 128);
-#pragma unroll
-            for (uint32_t i = 0; i < DW; i++) {
-                uint32_t f[4][4];  // d, d + 1, d + 2, d + 3 by position pairs
-#pragma unroll
-                for (uint32_t p = 0; p < 4; p++) {
-                    const uint32_t w0 = vw[2 * p][i], w1 = vw[2 * p + 1][i];
-                    const uint32_t x = __byte_perm(w0, w1, 0x5410), y = __byte_perm(w0, w1, 0x7632);
-                    f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x), f[2][p] = even_bytes(y), f[3][p] = odd_bytes(y);
+            if constexpr (!G::FOLD) {
+                if (lane < 16) {  // scales go with V: they are read until the weights are written
+                    sc[b * 2 * KT + 16 * cw + lane] = ks_now;
+                    sc[b * 2 * KT + KT + 16 * cw + lane] = vs_now;
                 }
+            }
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) {
-                    const uint32_t d = vd + 4 * i + e;
-                    *reinterpret_cast<uint4*>(vt + d * 128 + ((vg % 8) ^ (d & 7)) * 16) = make_uint4(f[e][0], f[e][1], f[e][2], f[e][3]);
+            for (uint32_t v = 0; v < VP; v++) {
+                uint32_t h[4];
+                if constexpr (G::FOLD) {
+#pragma unroll
+                    for (uint32_t p = 0; p < 4; p++) h[p] = __shfl_sync(0xffffffffu, vh, 4 * (VP == 2 ? v : lane / DW) + p);
+                }
+                // elements d, d + 1, then d + 2, d + 3, by position pairs; group
+                // vg + 1's pieces lie beside group vg's: vg is even there
+                const uint32_t to = (to_v ^ (16 * v)) + b * G::V_BYTES;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e += 2) {
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (uint32_t p = 0; p < 4; p++) {
+                        const uint32_t x = __byte_perm(vw[v][2 * p], vw[v][2 * p + 1], e == 0 ? 0x5410 : 0x7632);
+                        f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x);
+                        if constexpr (G::FOLD) f[0][p] = times(f[0][p], h[p]), f[1][p] = times(f[1][p], h[p]);
+                    }
+                    sts128(to + e * (DW * 128), make_uint4(f[0][0], f[0][1], f[0][2], f[0][3]));
+                    sts128(to + (e + 1) * (DW * 128), make_uint4(f[1][0], f[1][1], f[1][2], f[1][3]));
                 }
             }
             fence_proxy_async_smem();
-            mbar_arrive(&vfull[b]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&vfull[b]);
             if (t + 1 < tiles) load_v(t + 1);
-            bar_sync(3);  // vtop is free
         }
     } else {
         // ---------------------------------------------------- one row tile
-        tc5::setmaxnreg_inc<kChunkRegsRow>();
         const uint32_t w = warp / 4, th = tid % 128, row = w * 128 + th;
         if (w < users) {
             const bool on = row < live;
-            const uint64_t f = f0 + row;
+            const uint64_t f = f0 + (on ? row : 0);
             const uint32_t j = (uint32_t)(f / group), h = kvh * group + (uint32_t)(f - (uint64_t)j * group);
             const uint64_t p = (uint64_t)pos0 + j;
             const int lim = on && p < a.kv.max_ctx ? (int)p : -1;  // the last position this row sees
+            row_q[row] = (r0 + (uint64_t)j) * a.q.row + (uint64_t)h * a.q.head;
+            row_out[row] = (r0 + (uint64_t)j) * a.out.row + (uint64_t)h * a.out.head;
+            __syncwarp();
             uint8_t* qt = smem + G::Q_AT + w * G::Q_BYTES;
-            float cf;
-            {
-                // q to f16 rows of 64, elements 0, 2, 1, 3 of every four as K's codes lie
-                const uint64_t at = (r0 + (uint64_t)j) * a.q.row + (uint64_t)h * a.q.head;
-                float top = 0.0f;
-                if (on)
-                    for (uint32_t d = 0; d < HD; d++) top = fmaxf(top, fabsf(load1<DT>(a.q.p, at + d)));
-                float inv;
-                const float fit = fit_f16(top, &inv);
-                cf = (a.scale * kLog2e) * inv;
-#pragma unroll 4
-                for (uint32_t c = 0; c < HD / 8; c++) {
-                    float x[8];
+            // q to f16 rows of 64, elements 0, 2, 1, 3 of every four as K's codes
+            // lie; HD / 8 lanes take a row, eight elements each
+            constexpr uint32_t LPR = HD / 8, RPW = 32 / LPR, AT_ONCE = 8;
+            const uint32_t qc = lane % LPR;
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < LPR; i0 += AT_ONCE) {
+                float x[AT_ONCE][8];
+#pragma unroll
+                for (uint32_t i = 0; i < AT_ONCE; i++) {
+                    const uint64_t at = row_q[w * 128 + th / 32 * 32 + (i0 + i) * RPW + lane / LPR] + 8 * qc;
+                    load4<DT>(a.q.p, at, a.q_vec, x[i]);
+                    load4<DT>(a.q.p, at + 4, a.q_vec, x[i] + 4);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < AT_ONCE; i++) {
+                    const uint32_t r = th / 32 * 32 + (i0 + i) * RPW + lane / LPR;
+                    float top = 0.0f;
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[i][e]));
+#pragma unroll
+                    for (uint32_t d = LPR / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    float inv;
+                    const float fit = fit_f16(top, &inv);
+                    if (qc == 0) row_cf[w * 128 + r] = (a.scale * kLog2e) * inv;
                     uint32_t hi4[4], lo4[4];
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; e++) x[e] = on ? load1<DT>(a.q.p, at + 8 * c + e) * fit : 0.0f;
-#pragma unroll
                     for (uint32_t e = 0; e < 2; e++) {
-                        pair16(x[4 * e], x[4 * e + 2], &hi4[2 * e], &lo4[2 * e]);
-                        pair16(x[4 * e + 1], x[4 * e + 3], &hi4[2 * e + 1], &lo4[2 * e + 1]);
+                        pair16(x[i][4 * e] * fit, x[i][4 * e + 2] * fit, &hi4[2 * e], &lo4[2 * e]);
+                        pair16(x[i][4 * e + 1] * fit, x[i][4 * e + 3] * fit, &hi4[2 * e + 1], &lo4[2 * e + 1]);
                     }
-                    uint8_t* to = qt + c / 8 * G::SLAB + th * 128 + ((c % 8) ^ (th & 7)) * 16;
+                    uint8_t* to = qt + qc / 8 * G::SLAB + r * 128 + ((qc % 8) ^ (r & 7)) * 16;
                     *reinterpret_cast<uint4*>(to) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
                     if constexpr (G::QPAIR) *reinterpret_cast<uint4*>(to + 2 * G::Q_BYTES) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
                 }
             }
+            __syncwarp();
+            float kunit = 1.0f;
+            if constexpr (G::FOLD) fit_under(ktop, 7, &kunit);
+            const float cf = row_cf[row] * kunit;
             fence_proxy_async_smem();
             bar_sync(1 + w);
 
             const uint32_t scol = tmem + G::S_COL + w * KT, ocol = tmem + G::O_COL + w * HD;
             const uint32_t lanes = (warp % 4 * 32) << 16;
+            // the tile's operands, as descriptors
+            const uint64_t q_desc = tc5::sw128_desc(smem_u32(qt)), k_desc = tc5::sw128_desc(smem_u32(smem + G::K_AT)),
+                           v_desc = tc5::sw128_desc(smem_u32(smem + G::V_AT));
             auto issue_s = [&](uint32_t t) {
                 const uint32_t b = t % NB;
                 wait(&kfull[b], t / NB & 1);
                 tc5::fence_after();
-                const uint32_t kb = smem_u32(smem + G::K_AT + b * G::K_BYTES), qb = smem_u32(qt);
+                if (tc5::elect()) {
+                    const uint64_t kd = k_desc + b * (G::K_BYTES / 16);
 #pragma unroll
-                for (uint32_t k = 0; k < HD / 16; k++) {
-                    const uint64_t kd = tc5::sw128_desc(kb + k / 4 * G::SLAB) + 2 * (k % 4);
-                    const uint64_t qd = tc5::sw128_desc(qb + k / 4 * G::SLAB) + 2 * (k % 4);
-                    if constexpr (G::QPAIR) {
-                        const uint64_t ld = tc5::sw128_desc(qb + 2 * G::Q_BYTES + k / 4 * G::SLAB) + 2 * (k % 4);
-                        tc5::mma_ss(scol, ld, kd, tc5::idesc_f16(128, KT), k > 0);
-                        tc5::mma_ss(scol, qd, kd, tc5::idesc_f16(128, KT), true);
-                    } else {
-                        tc5::mma_ss(scol, qd, kd, tc5::idesc_f16(128, KT), k > 0);
+                    for (uint32_t k = 0; k < HD / 16; k++) {
+                        const uint32_t at = k / 4 * (G::SLAB / 16) + 2 * (k % 4);
+                        if constexpr (G::QPAIR) tc5::mma_ss(scol, q_desc + 2 * G::Q_BYTES / 16 + at, kd + at, tc5::idesc_f16(128, KT), k > 0);
+                        tc5::mma_ss(scol, q_desc + at, kd + at, tc5::idesc_f16(128, KT), G::QPAIR || k > 0);
                     }
+                    tc5::commit(&s_done[w]);
+                    tc5::commit(&kempty[b]);
                 }
-                tc5::commit(&s_done[w]);
-                tc5::commit(&kempty[b]);
+                __syncwarp();
             };
             auto issue_o = [&](uint32_t t) {
                 const uint32_t b = t % NB;
-                wait(&vfull[b], t / NB & 1);
                 tc5::fence_after();
-                const uint32_t vb = smem_u32(smem + G::V_AT + b * G::V_BYTES);
+                if (tc5::elect()) {
+                    const uint64_t vd = v_desc + b * (G::V_BYTES / 16);
+                    const bool more = t > 0;
 #pragma unroll
-                for (uint32_t k = 0; k < KT / 16; k++) {
-                    const uint64_t vd = tc5::sw128_desc(vb + k / 4 * (HD * 128)) + 2 * (k % 4);
-                    const uint32_t wc = scol + k / 2 * 32 + k % 2 * 8;
-                    if constexpr (G::WPAIR) {
-                        tc5::mma_ts(ocol, wc + 16, vd, tc5::idesc_f16(128, HD), k > 0);
-                        tc5::mma_ts(ocol, wc, vd, tc5::idesc_f16(128, HD), true);
-                    } else {
-                        tc5::mma_ts(ocol, wc, vd, tc5::idesc_f16(128, HD), k > 0);
+                    for (uint32_t k = 0; k < KT / 16; k++) {
+                        const uint32_t at = k / 4 * (HD * 128 / 16) + 2 * (k % 4);
+                        if constexpr (G::WPAIR) tc5::mma_ts(ocol, scol + k * 16 + 8, vd + at, tc5::idesc_f16(128, HD), k > 0 || more);
+                        tc5::mma_ts(ocol, scol + k * 16, vd + at, tc5::idesc_f16(128, HD), G::WPAIR || k > 0 || more);
                     }
+                    tc5::commit(&o_done[w]);
+                    tc5::commit(&vempty[b]);
                 }
-                tc5::commit(&o_done[w]);
-                tc5::commit(&vempty[b]);
+                __syncwarp();
             };
-            if (th == 0) issue_s(0);
+            const bool issuer = warp % 4 == 0;
+            if (issuer) issue_s(0);
 
-            float o[HD], mx = -INFINITY, l = 0.0f, alpha = 1.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < HD; i++) o[i] = 0.0f;
-            auto add_o = [&](uint32_t t) {  // the outputs of tile t, once they are there
-                wait(&o_done[w], t & 1);
-                tc5::fence_after();
-#pragma unroll
-                for (uint32_t c = 0; c < HD / 32; c++) {
-                    float x[32];
-                    tc5::ld32(ocol + lanes + 32 * c, x);
-                    tc5::wait_ld();
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; i++) o[32 * c + i] = fmaf(o[32 * c + i], alpha, x[i]);
-                }
-            };
-            for (uint32_t t = 0; t < tiles; t++) {
-                const uint32_t b = t % NB;
-                const float* ks = sc + b * 2 * KT;
-                const int left = lim - (int)(t * KT);  // columns 0..left are seen
-                const bool full = __all_sync(0xffffffffu, left >= (int)KT - 1);
-                wait(&vfull[b], t / NB & 1);
-                wait(&s_done[w], t & 1);
-                tc5::fence_after();
-                float s[G::HOLD ? KT : 32], top = -INFINITY;
-                auto scores = [&](uint32_t c, float* x) {  // columns 32 c.. under K's scales, unseen ones -inf
-                    tc5::ld32(scol + lanes + 32 * c, x);
-                    tc5::wait_ld();
+            float mx = -INFINITY, l = 0.0f;  // the running maximum in powers of two
+            // Columns 32 c.. of the scores, under K's scales where these are outside.
+            auto scaled = [&](const float* ks, uint32_t c, float* x) {
+                if constexpr (!G::FOLD) {
 #pragma unroll
                     for (uint32_t i = 0; i < 32; i += 4) {
                         const float4 k4 = *reinterpret_cast<const float4*>(ks + 32 * c + i);
-                        x[i] *= k4.x, x[i + 1] *= k4.y, x[i + 2] *= k4.z, x[i + 3] *= k4.w;
+                        mul2(x + i, k4.x, k4.y);
+                        mul2(x + i + 2, k4.z, k4.w);
                     }
-                    if (!full) {
+                }
+            };
+            auto largest = [&](auto masked, uint32_t c, const float* x, float top, int left) {
 #pragma unroll
-                        for (uint32_t i = 0; i < 32; i++)
-                            if ((int)(32 * c + i) > left) x[i] = -INFINITY;
+                for (uint32_t i = 0; i < 32; i++) {
+                    if constexpr (decltype(masked)::value) {
+                        if ((int)(32 * c + i) <= left) top = fmaxf(top, x[i]);
+                    } else {
+                        top = fmaxf(top, x[i]);
                     }
-                };
-#pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
-                    float* x = s + (G::HOLD ? 32 * c : 0);
-                    scores(c, x);
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; i++) top = fmaxf(top, x[i]);
                 }
-                if (t > 0) add_o(t - 1);
-                alpha = 1.0f;
-                if ((top - mx) * cf > kSlack) {
-                    alpha = ex2((mx - top) * cf);
-                    mx = top;
-                    l *= alpha;
-                }
-                const float off = mx == -INFINITY ? 0.0f : -mx * cf;
-                alpha *= vratio[b];
-                const float* vs = ks + KT;
-                float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                return top;
+            };
+            // Weights of columns 32 c.. into TMEM over their scores (of each 16, hi in
+            // the first eight columns, lo in the others); returns their sum.
+            auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left) {
+                float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
-                    float* x = s + (G::HOLD ? 32 * c : 0);
-                    if constexpr (!G::HOLD) scores(c, x);
-                    uint32_t wh[16], wl[16];
+                for (uint32_t k = 0; k < 32; k += 16) {
+                    uint32_t wh[8], wl[8];
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; i += 4) {
-                        const float4 v4 = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-                        const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-                        float y[4];
+                    for (uint32_t i = k; i < k + 16; i += 4) {
+                        fma2(x + i, cf, off);
+                        fma2(x + i + 2, cf, off);
 #pragma unroll
                         for (uint32_t e = 0; e < 4; e++) {
-                            const bool out = !full && (int)(32 * c + i + e) > left;
-                            const float pr = out ? 0.0f : ex2(fmaf(x[i + e], cf, off));
-                            l4[e] += pr;
-                            y[e] = out ? 0.0f : pr * v[e];  // a scale of NaN does not reach rows before it
+                            x[i + e] = ex2(x[i + e]);
+                            if constexpr (decltype(masked)::value)
+                                if ((int)(32 * c + i + e) > left) x[i + e] = 0.0f;
                         }
-                        pair16(y[0], y[1], &wh[i / 2], &wl[i / 2]);
-                        pair16(y[2], y[3], &wh[i / 2 + 1], &wl[i / 2 + 1]);
+                        add2(sum, x + i);
+                        add2(sum, x + i + 2);
+                        if constexpr (!G::FOLD) {
+                            const float4 v4 = *reinterpret_cast<const float4*>(vs + 32 * c + i);
+                            mul2(x + i, v4.x, v4.y);
+                            mul2(x + i + 2, v4.z, v4.w);
+                            if constexpr (decltype(masked)::value) {  // a scale of NaN does not reach rows before it
+#pragma unroll
+                                for (uint32_t e = 0; e < 4; e++)
+                                    if ((int)(32 * c + i + e) > left) x[i + e] = 0.0f;
+                            }
+                        }
+                        pair16(x[i], x[i + 1], &wh[(i - k) / 2], &wl[(i - k) / 2]);
+                        pair16(x[i + 2], x[i + 3], &wh[(i - k) / 2 + 1], &wl[(i - k) / 2 + 1]);
                     }
-                    tc5::st16(scol + lanes + 32 * c, wh);
-                    if constexpr (G::WPAIR) tc5::st16(scol + lanes + 32 * c + 16, wl);
+                    tc5::st8(scol + lanes + 32 * c + k, wh);
+                    if constexpr (G::WPAIR) tc5::st8(scol + lanes + 32 * c + k + 8, wl);
                 }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                return sum[0] + sum[1];
+            };
+            // One tile: the scores are read twice, for their maximum and for the
+            // weights, so that few registers hold them; the next columns are on
+            // their way from TMEM while these are worked on.
+            auto tile = [&](auto masked, uint32_t t, int left) {
+                const float *ks = sc + t % NB * 2 * KT, *vs = ks + KT;
+                float top = -INFINITY, x[2][32];
+                tc5::ld32(scol + lanes, x[0]);
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    tc5::wait_ld();
+                    tc5::ld32(scol + lanes + 32 * ((c + 1) % 4), x[(c + 1) % 2]);  // at last the first again
+                    scaled(ks, c, x[c % 2]);
+                    top = largest(masked, c, x[c % 2], top, left);
+                }
+                top *= cf;
+                const bool up = top > mx + kSlack;
+                const float alpha = up ? ex2(mx - top) : 1.0f;
+                l *= alpha;
+                mx = up ? top : mx;
+                if (t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum
+                    tc5::wait_ld();
+                    wait(&o_done[w], (t - 1) & 1);
+                    tc5::fence_after();
+#pragma unroll
+                    for (uint32_t c = 0; c < HD / 16; c++) {
+                        float y[16];
+                        tc5::ld16(ocol + lanes + 16 * c, y);
+                        tc5::wait_ld();
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i++) y[i] *= alpha;
+                        tc5::st16(ocol + lanes + 16 * c, reinterpret_cast<const uint32_t*>(y));
+                    }
+                }
+                const float off = (mx == -INFINITY ? 0.0f : -mx) + G::PEXP;
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < 4; c++) {
+                    tc5::wait_ld();
+                    if (c < 3) tc5::ld32(scol + lanes + 32 * (c + 1), x[(c + 1) % 2]);
+                    scaled(ks, c, x[c % 2]);
+                    sum += weights(masked, vs, c, x[c % 2], off, left);
+                }
+                l += sum;
+            };
+            for (uint32_t t = 0; t < tiles; t++) {
+                const int left = lim - (int)(t * KT);  // columns 0..left are seen
+                wait(&vfull[t % NB], t / NB & 1);
+                wait(&s_done[w], t & 1);
+                tc5::fence_after();
+                if (__all_sync(0xffffffffu, left >= (int)KT - 1)) tile(std::false_type{}, t, left);
+                else tile(std::true_type{}, t, left);
                 tc5::wait_st();
                 tc5::fence_before();
                 bar_sync(1 + w);
-                if (th == 0) {
-                    tc5::fence_after();
+                if (issuer) {
                     issue_o(t);
                     if (t + 1 < tiles) issue_s(t + 1);
                 }
-                __syncwarp();
             }
-            add_o(tiles - 1);
-            if (on) {
-                const float unit = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
-                const uint64_t at = (r0 + (uint64_t)j) * a.out.row + (uint64_t)h * a.out.head;
+            wait(&o_done[w], (tiles - 1) & 1);
+            tc5::fence_after();
+            // rows out, 32 columns at a time through the warp's share of q's space:
+            // a float4 q of row r lies at r * 8 + (q ^ r % 8)
+            float vunit;
+            fit_under(vtop, G::VEXP, &vunit);
+            const float unit = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
+            // column e * HD / 4 + i of O' is element 4 i + e
+            float4* stage = reinterpret_cast<float4*>(qt + warp % 4 * 4096);
+            bar_sync(1 + w);
 #pragma unroll
-                for (uint32_t i = 0; i < HD; i++) store1<DT>(const_cast<void*>(a.out.p), at + i, lim >= 0 ? o[i] * unit : 0.0f);
+            for (uint32_t c = 0; c < HD / 32; c++) {
+                float y[4][8];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) tc5::ld8(ocol + lanes + e * (HD / 4) + 8 * c, y[e]);
+                tc5::wait_ld();
+#pragma unroll
+                for (uint32_t q = 0; q < 8; q++) {
+                    float4 v = make_float4(y[0][q] * unit, y[1][q] * unit, y[2][q] * unit, y[3][q] * unit);
+                    if (lim < 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    stage[lane * 8 + (q ^ (lane & 7))] = v;
+                }
+                __syncwarp();
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    const uint32_t r = 4 * i + lane / 8, q = lane % 8, at = w * 128 + th / 32 * 32 + r;
+                    if (at < live)
+                        store4<DT>(const_cast<void*>(a.out.p), row_out[at] + 32 * c + 4 * q, a.out_vec, stage[r * 8 + (q ^ (r & 7))]);
+                }
+                __syncwarp();
             }
         }
     }
@@ -960,10 +1145,6 @@ cudaError_t set_limits() {
         e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 2>::RING);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_kv8_chunk<HD, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkGeom<HD, DT>::BYTES);
-    // the chunk kernel deals the registers of its launch out anew: all of them must be there
-    cudaFuncAttributes at{};
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, k_kv8_chunk<HD, DT>);
-    if (e == cudaSuccess && at.numRegs * 3 < kChunkRegsRow * 2 + kChunkRegsCode) e = cudaErrorInvalidConfiguration;
     return e;
 }
 

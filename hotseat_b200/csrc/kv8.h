@@ -122,6 +122,7 @@ struct Kv8AttendArgs {
     Kv8Mat q, out;
     uint32_t nh = 0, group = 0, chunks = 0;  // query heads, per KV head, and CTAs of kv8_single_cols for these
     float scale = 1.0f;
+    bool q_vec = false, out_vec = false;  // four elements of a row at once: base and strides allow it
     // single rows: CTAs of `cluster` splits join in shared memory; where a
     // region's rows can need more of them, their records [slot][KV head][head
     // chunk][max_clusters][kv8_record] and, for each (slot, KV head, chunk),

@@ -103,6 +103,12 @@ Kv8Rows rows_of(const hs_kv8_set* s, uint32_t n_rows, const uint32_t* row_start,
     return r;
 }
 
+// Whether four consecutive elements of a row can be taken at once.
+bool fours(const Kv8Mat& m) {
+    const uint64_t b = 4 * dtype_bytes(m.dtype);
+    return reinterpret_cast<uintptr_t>(m.p) % b == 0 && m.row % 4 == 0 && m.head % 4 == 0;
+}
+
 int launched(cudaError_t e, const char* what) {
     return e == cudaSuccess ? HS_OK : fail(HS_E_CUDA, std::string(what) + " launch: " + cudaGetErrorString(e));
 }
@@ -275,6 +281,8 @@ int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t
     a.group = s->nh / s->spec.n_kv_heads;
     a.chunks = (a.group + kv8_single_cols(a.group) - 1) / kv8_single_cols(a.group);
     a.scale = scale;
+    a.q_vec = fours(a.q);
+    a.out_vec = fours(a.out);
     a.part = s->part;
     a.counters = s->counters;
     a.max_splits = s->max_splits;
