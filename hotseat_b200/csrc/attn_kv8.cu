@@ -955,12 +955,12 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
             if (issuer) issue_s(0);
 
             float mx = -INFINITY, l = 0.0f;  // the running maximum in powers of two
-            // Columns 32 c.. of the scores, under K's scales where these are outside.
+            // Columns 16 c.. of the scores, under K's scales where these are outside.
             auto scaled = [&](const float* ks, uint32_t c, float* x) {
                 if constexpr (!G::FOLD) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; i += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4*>(ks + 32 * c + i);
+                    for (uint32_t i = 0; i < 16; i += 4) {
+                        const float4 k4 = *reinterpret_cast<const float4*>(ks + 16 * c + i);
                         mul2(x + i, k4.x, k4.y);
                         mul2(x + i + 2, k4.z, k4.w);
                     }
@@ -968,65 +968,64 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
             };
             auto largest = [&](auto masked, uint32_t c, const float* x, float top, int left) {
 #pragma unroll
-                for (uint32_t i = 0; i < 32; i++) {
+                for (uint32_t i = 0; i < 16; i++) {
                     if constexpr (decltype(masked)::value) {
-                        if ((int)(32 * c + i) <= left) top = fmaxf(top, x[i]);
+                        if ((int)(16 * c + i) <= left) top = fmaxf(top, x[i]);
                     } else {
                         top = fmaxf(top, x[i]);
                     }
                 }
                 return top;
             };
-            // Weights of columns 32 c.. into TMEM over their scores (of each 16, hi in
-            // the first eight columns, lo in the others); returns their sum.
-            auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left) {
-                float sum[2] = {0.0f, 0.0f};
+            // Weights of columns 16 c.. into TMEM over their scores (hi in the first
+            // eight columns, lo in the others); adds their sum.
+            auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left, float* sum) {
+                uint32_t wh[8], wl[8];
 #pragma unroll
-                for (uint32_t k = 0; k < 32; k += 16) {
-                    uint32_t wh[8], wl[8];
+                for (uint32_t i = 0; i < 16; i += 4) {
+                    fma2(x + i, cf, off);
+                    fma2(x + i + 2, cf, off);
 #pragma unroll
-                    for (uint32_t i = k; i < k + 16; i += 4) {
-                        fma2(x + i, cf, off);
-                        fma2(x + i + 2, cf, off);
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; e++) {
-                            x[i + e] = ex2(x[i + e]);
-                            if constexpr (decltype(masked)::value)
-                                if ((int)(32 * c + i + e) > left) x[i + e] = 0.0f;
-                        }
-                        add2(sum, x + i);
-                        add2(sum, x + i + 2);
-                        if constexpr (!G::FOLD) {
-                            const float4 v4 = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-                            mul2(x + i, v4.x, v4.y);
-                            mul2(x + i + 2, v4.z, v4.w);
-                            if constexpr (decltype(masked)::value) {  // a scale of NaN does not reach rows before it
-#pragma unroll
-                                for (uint32_t e = 0; e < 4; e++)
-                                    if ((int)(32 * c + i + e) > left) x[i + e] = 0.0f;
-                            }
-                        }
-                        pair16(x[i], x[i + 1], &wh[(i - k) / 2], &wl[(i - k) / 2]);
-                        pair16(x[i + 2], x[i + 3], &wh[(i - k) / 2 + 1], &wl[(i - k) / 2 + 1]);
+                    for (uint32_t e = 0; e < 4; e++) {
+                        x[i + e] = ex2(x[i + e]);
+                        if constexpr (decltype(masked)::value)
+                            if ((int)(16 * c + i + e) > left) x[i + e] = 0.0f;
                     }
-                    tc5::st8(scol + lanes + 32 * c + k, wh);
-                    if constexpr (G::WPAIR) tc5::st8(scol + lanes + 32 * c + k + 8, wl);
+                    add2(sum, x + i);
+                    add2(sum, x + i + 2);
+                    if constexpr (!G::FOLD) {
+                        const float4 v4 = *reinterpret_cast<const float4*>(vs + 16 * c + i);
+                        mul2(x + i, v4.x, v4.y);
+                        mul2(x + i + 2, v4.z, v4.w);
+                        if constexpr (decltype(masked)::value) {  // a scale of NaN does not reach rows before it
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; e++)
+                                if ((int)(16 * c + i + e) > left) x[i + e] = 0.0f;
+                        }
+                    }
+                    pair16(x[i], x[i + 1], &wh[i / 2], &wl[i / 2]);
+                    pair16(x[i + 2], x[i + 3], &wh[i / 2 + 1], &wl[i / 2 + 1]);
                 }
-                return sum[0] + sum[1];
+                tc5::st8(scol + lanes + 16 * c, wh);
+                if constexpr (G::WPAIR) tc5::st8(scol + lanes + 16 * c + 8, wl);
             };
             // One tile: the scores are read twice, for their maximum and for the
             // weights, so that few registers hold them; the next columns are on
             // their way from TMEM while these are worked on.
             auto tile = [&](auto masked, uint32_t t, int left) {
                 const float *ks = sc + t % NB * 2 * KT, *vs = ks + KT;
-                float top = -INFINITY, x[2][32];
-                tc5::ld32(scol + lanes, x[0]);
-#pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
+                float top = -INFINITY, x[16], y[16];
+                tc5::ld16(scol + lanes, x);
+#pragma unroll 1
+                for (uint32_t c = 0; c < 8; c += 2) {
                     tc5::wait_ld();
-                    tc5::ld32(scol + lanes + 32 * ((c + 1) % 4), x[(c + 1) % 2]);  // at last the first again
-                    scaled(ks, c, x[c % 2]);
-                    top = largest(masked, c, x[c % 2], top, left);
+                    tc5::ld16(scol + lanes + 16 * (c + 1), y);
+                    scaled(ks, c, x);
+                    top = largest(masked, c, x, top, left);
+                    tc5::wait_ld();
+                    tc5::ld16(scol + lanes + 16 * ((c + 2) % 8), x);  // at last the first again
+                    scaled(ks, c + 1, y);
+                    top = largest(masked, c + 1, y, top, left);
                 }
                 top *= cf;
                 const bool up = top > mx + kSlack;
@@ -1037,9 +1036,8 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                     tc5::wait_ld();
                     wait(&o_done[w], (t - 1) & 1);
                     tc5::fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (uint32_t c = 0; c < HD / 16; c++) {
-                        float y[16];
                         tc5::ld16(ocol + lanes + 16 * c, y);
                         tc5::wait_ld();
 #pragma unroll
@@ -1048,15 +1046,19 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                     }
                 }
                 const float off = (mx == -INFINITY ? 0.0f : -mx) + G::PEXP;
-                float sum = 0.0f;
-#pragma unroll
-                for (uint32_t c = 0; c < 4; c++) {
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+                for (uint32_t c = 0; c < 8; c += 2) {
                     tc5::wait_ld();
-                    if (c < 3) tc5::ld32(scol + lanes + 32 * (c + 1), x[(c + 1) % 2]);
-                    scaled(ks, c, x[c % 2]);
-                    sum += weights(masked, vs, c, x[c % 2], off, left);
+                    tc5::ld16(scol + lanes + 16 * (c + 1), y);
+                    scaled(ks, c, x);
+                    weights(masked, vs, c, x, off, left, sum);
+                    tc5::wait_ld();
+                    if (c < 6) tc5::ld16(scol + lanes + 16 * (c + 2), x);
+                    scaled(ks, c + 1, y);
+                    weights(masked, vs, c + 1, y, off, left, sum);
                 }
-                l += sum;
+                l += sum[0] + sum[1];
             };
             for (uint32_t t = 0; t < tiles; t++) {
                 const int left = lim - (int)(t * KT);  // columns 0..left are seen
@@ -1075,35 +1077,41 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
             }
             wait(&o_done[w], (tiles - 1) & 1);
             tc5::fence_after();
-            // rows out, 32 columns at a time through the warp's share of q's space:
-            // a float4 q of row r lies at r * 8 + (q ^ r % 8)
+            // what a row's outputs are divided by goes through shared memory: the
+            // registers of this loop stay its own (rows that see nothing: sums of 0)
             float vunit;
             fit_under(vtop, G::VEXP, &vunit);
-            const float unit = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
-            // column e * HD / 4 + i of O' is element 4 i + e
-            float4* stage = reinterpret_cast<float4*>(qt + warp % 4 * 4096);
-            bar_sync(1 + w);
+            row_cf[row] = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
+        }
+    }
+    __syncwarp();
+    if (warp < 4 * users) {
+        // Rows out, 32 columns at a time through the warp's share of q's space:
+        // a float4 q of row r lies at r * 8 + (q ^ r % 8). Column e * HD / 4 + i
+        // of O' is element 4 i + e. (Every product that reads q is done: the
+        // tile's last outputs are.)
+        const uint32_t w = warp / 4, row0 = warp * 32;
+        const float unit = row_cf[row0 + lane];
+        float4* stage = reinterpret_cast<float4*>(smem + G::Q_AT + w * G::Q_BYTES + warp % 4 * 4096);
+        const uint32_t oc = tmem + G::O_COL + w * HD + ((warp % 4 * 32) << 16);
+        bar_sync(1 + w);
+#pragma unroll 1
+        for (uint32_t c = 0; c < HD / 32; c++) {
+            float y[4][8];
 #pragma unroll
-            for (uint32_t c = 0; c < HD / 32; c++) {
-                float y[4][8];
+            for (uint32_t e = 0; e < 4; e++) tc5::ld8(oc + e * (HD / 4) + 8 * c, y[e]);
+            tc5::wait_ld();
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) tc5::ld8(ocol + lanes + e * (HD / 4) + 8 * c, y[e]);
-                tc5::wait_ld();
+            for (uint32_t q = 0; q < 8; q++)
+                stage[lane * 8 + (q ^ (lane & 7))] = make_float4(y[0][q] * unit, y[1][q] * unit, y[2][q] * unit, y[3][q] * unit);
+            __syncwarp();
 #pragma unroll
-                for (uint32_t q = 0; q < 8; q++) {
-                    float4 v = make_float4(y[0][q] * unit, y[1][q] * unit, y[2][q] * unit, y[3][q] * unit);
-                    if (lim < 0) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    stage[lane * 8 + (q ^ (lane & 7))] = v;
-                }
-                __syncwarp();
-#pragma unroll
-                for (uint32_t i = 0; i < 8; i++) {
-                    const uint32_t r = 4 * i + lane / 8, q = lane % 8, at = w * 128 + th / 32 * 32 + r;
-                    if (at < live)
-                        store4<DT>(const_cast<void*>(a.out.p), row_out[at] + 32 * c + 4 * q, a.out_vec, stage[r * 8 + (q ^ (r & 7))]);
-                }
-                __syncwarp();
+            for (uint32_t i = 0; i < 8; i++) {
+                const uint32_t r = 4 * i + lane / 8, q = lane % 8;
+                if (row0 + r < live)
+                    store4<DT>(const_cast<void*>(a.out.p), row_out[row0 + r] + 32 * c + 4 * q, a.out_vec, stage[r * 8 + (q ^ (r & 7))]);
             }
+            __syncwarp();
         }
     }
     tc5::fence_before();
