@@ -568,7 +568,13 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 template <int HD, int DT>
 struct ChunkGeom {
     static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
-    static constexpr uint32_t KT = 128, ROWS = 256, THREADS = 512;
+    static constexpr uint32_t KT = 128, ROWS = 256;
+    // f32 rows take each tile's O' out of TMEM and sum it in registers, rounded
+    // to nearest: left to grow there, 2,048 positions were 1.7e-6 off (the
+    // tensor cores' sums truncate), so 5e-7. Their row warps get 192 registers a
+    // thread, and four code warps, of 120, do with the rest.
+    static constexpr bool OREG = DT == HS_F32;
+    static constexpr uint32_t CW = OREG ? 4 : 8, THREADS = 256 + 32 * CW, SUB = 8 / CW;
     static constexpr uint32_t SLAB = 128 * 128;            // 128 rows of 64 f16
     static constexpr uint32_t Q_BYTES = HD / 64 * SLAB;    // one row tile, hi or lo
     static constexpr uint32_t K_BYTES = HD / 64 * SLAB, V_BYTES = 2 * HD * 128;
@@ -588,6 +594,10 @@ struct ChunkGeom {
 };
 
 constexpr uint32_t kChunkLimit = 1u << 22;
+// Registers a thread of the row warps and of the code warps where they are
+// dealt out anew: two of the first and one of the second are what the launch
+// of 384 threads holds, 168 a thread.
+constexpr int kChunkRegsRow = 192, kChunkRegsCode = 120;
 
 // Two f32 at once (each rounded on its own).
 __device__ __forceinline__ void mul2(float* x, float a, float b) {
@@ -618,7 +628,7 @@ __device__ __forceinline__ void bar_sync(uint32_t id) {
 }
 
 template <int HD, int DT>
-__global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
+__global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(const Kv8AttendArgs a) {
     using G = ChunkGeom<HD, DT>;
     constexpr uint32_t KT = G::KT, NB = G::NB;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -666,8 +676,8 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
 
     if (tid == 0) {
         for (uint32_t i = 0; i < NB; i++) {
-            mbar_init(&kfull[i], 8);  // a warp's arrival each
-            mbar_init(&vfull[i], 8);
+            mbar_init(&kfull[i], G::CW);  // a warp's arrival each
+            mbar_init(&vfull[i], G::CW);
             mbar_init(&kempty[i], users);
             mbar_init(&vempty[i], users);
         }
@@ -706,7 +716,7 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
     auto fit_under = [](const float* tops, uint32_t exp, float* inverse) {
         float top = 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < 16; i++) top = fmaxf(top, tops[i]);
+        for (uint32_t i = 0; i < G::THREADS / 32; i++) top = fmaxf(top, tops[i]);
         const uint32_t e = top > 0.0f ? min((__float_as_uint(top) >> 23) + 1, 253u) : 127u + exp;
         const uint32_t bits = min(254u + exp - e, 253u);
         *inverse = __uint_as_float((254u - bits) << 23);
@@ -725,7 +735,10 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
 
     if (warp >= 8) {
         // ---------------------------------------------------- codes to f16
-        const uint32_t cw = warp - 8;  // this warp's positions of a tile: 16 cw .. 16 cw + 15
+        if constexpr (G::OREG) tc5::setmaxnreg_dec<kChunkRegsCode>();
+        // this warp's positions of a tile: 16 of each 128 / SUB, from 16 cw on
+        const uint32_t cw = warp - 8;
+        constexpr uint32_t SP = KT / G::SUB;
         const uint64_t ps = a.kv.pos_stride;
         // K: a lane takes 16 codes of rows kr, kr + RPP, ...
         constexpr uint32_t CPR = HD / 16, RPP = 32 / CPR, KP = 16 / RPP;
@@ -741,38 +754,38 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
         const uint32_t dw = lane % DW, vg = 2 * cw + lane / DW;
         const uint8_t* kp = base + a.kv.code_off(0, kvh, 0) + 16 * kc;
         const uint8_t* vp = base + a.kv.code_off(1, kvh, 0) + 4 * dw;
-        uint4 kw[KP];
-        uint32_t vw[VP][8];
-        float ks, vs;
-        auto load_k = [&](uint32_t t) {
-            const uint32_t p0 = t * KT + 16 * cw + kr;
+        uint4 kw[G::SUB][KP];
+        uint32_t vw[G::SUB][VP][8];
+        float ks[G::SUB], vs[G::SUB];
+        auto load_k = [&](uint32_t t, uint32_t u) {
+            const uint32_t p0 = t * KT + u * SP + 16 * cw + kr;
             if ((t + 1) * KT <= end) {
                 const uint8_t* q = kp + p0 * ps;
 #pragma unroll
-                for (uint32_t i = 0; i < KP; i++, q += RPP * ps) kw[i] = __ldg(reinterpret_cast<const uint4*>(q));
+                for (uint32_t i = 0; i < KP; i++, q += RPP * ps) kw[u][i] = __ldg(reinterpret_cast<const uint4*>(q));
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < KP; i++)
-                    kw[i] = __ldg(reinterpret_cast<const uint4*>(kp + min(p0 + i * RPP, end - 1) * ps));
+                    kw[u][i] = __ldg(reinterpret_cast<const uint4*>(kp + min(p0 + i * RPP, end - 1) * ps));
             }
         };
-        auto load_v = [&](uint32_t t) {
-            const uint32_t p0 = t * KT + 8 * vg;
+        auto load_v = [&](uint32_t t, uint32_t u) {
+            const uint32_t p0 = t * KT + u * SP + 8 * vg;
             if ((t + 1) * KT <= end) {
                 const uint8_t* q = vp + p0 * ps;
 #pragma unroll
-                for (uint32_t i = 0; i < VP * 8; i++, q += ps) vw[i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(q));
+                for (uint32_t i = 0; i < VP * 8; i++, q += ps) vw[u][i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(q));
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < VP * 8; i++)
-                    vw[i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(vp + min(p0 + i, end - 1) * ps));
+                    vw[u][i / 8][i % 8] = __ldg(reinterpret_cast<const uint32_t*>(vp + min(p0 + i, end - 1) * ps));
             }
         };
-        auto load_s = [&](uint32_t t) {  // position 16 cw + lane % 16; behind the end: 0
-            const uint32_t p = t * KT + 16 * cw + lane % 16;
+        auto load_s = [&](uint32_t t, uint32_t u) {  // the position of lane % 16; behind the end: 0
+            const uint32_t p = t * KT + u * SP + 16 * cw + lane % 16;
             const float* at = ksp + (uint64_t)(min(p, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride;
-            ks = p < end ? __ldg(at) * kfit : 0.0f;
-            vs = p < end ? __ldg(at + a.kv.splane / 4) * vfit : 0.0f;
+            ks[u] = p < end ? __ldg(at) * kfit : 0.0f;
+            vs[u] = p < end ? __ldg(at + a.kv.splane / 4) * vfit : 0.0f;
         };
         auto times = [](uint32_t x, uint32_t h) {
             const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&h));
@@ -782,83 +795,93 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
         // lies beside it), of the pieces' row dw (the others DW rows on)
         const uint32_t to_k = smem_u32(smem + G::K_AT) + kc / 4 * G::SLAB + (16 * cw + kr) * 128 + ((2 * kc % 8) ^ (kr & 7)) * 16;
         const uint32_t to_v = smem_u32(smem + G::V_AT) + vg / 8 * (HD * 128) + dw * 128 + ((vg % 8) ^ (dw & 7)) * 16;
-        load_s(0);
-        load_k(0);
-        load_v(0);
+#pragma unroll
+        for (uint32_t u = 0; u < G::SUB; u++) load_s(0, u), load_k(0, u), load_v(0, u);
         for (uint32_t t = 0; t < tiles; t++) {
             const uint32_t b = t % NB, use = t / NB;
-            uint32_t kh = 0, vh = 0;  // FOLD: position lane % 16's scale twice; positions 2 i, 2 i + 1 of lane i's
-            if constexpr (G::FOLD) {
-                // A NaN in either scale goes to the scores, where only the rows
-                // that see the position take it; V's row is then zeros.
-                const bool bad = isnan(vs);
-                const __half2 k2 = __float2half2_rn(bad ? vs : ks);
-                kh = *reinterpret_cast<const uint32_t*>(&k2);
-                const uint32_t v1 = __half_as_ushort(__float2half_rn(bad ? 0.0f : vs));
-                const uint32_t v0 = __shfl_sync(0xffffffffu, v1, 2 * lane), v2 = __shfl_sync(0xffffffffu, v1, 2 * lane + 1);
-                vh = v0 | v2 << 16;
+            uint32_t kh[G::SUB], vh[G::SUB];  // FOLD: position lane % 16's scale twice; positions 2 i, 2 i + 1 of lane i's
+            float ks_now[G::SUB], vs_now[G::SUB];
+#pragma unroll
+            for (uint32_t u = 0; u < G::SUB; u++) {
+                ks_now[u] = ks[u], vs_now[u] = vs[u];
+                if constexpr (G::FOLD) {
+                    // A NaN in either scale goes to the scores, where only the rows
+                    // that see the position take it; V's row is then zeros.
+                    const bool bad = isnan(vs[u]);
+                    const __half2 k2 = __float2half2_rn(bad ? vs[u] : ks[u]);
+                    kh[u] = *reinterpret_cast<const uint32_t*>(&k2);
+                    const uint32_t v1 = __half_as_ushort(__float2half_rn(bad ? 0.0f : vs[u]));
+                    const uint32_t v0 = __shfl_sync(0xffffffffu, v1, 2 * lane), v2 = __shfl_sync(0xffffffffu, v1, 2 * lane + 1);
+                    vh[u] = v0 | v2 << 16;
+                }
+                if (t + 1 < tiles) load_s(t + 1, u);
             }
-            const float ks_now = ks, vs_now = vs;
-            if (t + 1 < tiles) load_s(t + 1);
             if (use > 0) wait(&kempty[b], (use - 1) & 1);
 #pragma unroll
-            for (uint32_t i = 0; i < KP; i++) {
-                const uint4 w = kw[i];
-                // codes 0, 2, 1, 3 of every four, as q's elements lie
-                uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
-                uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
-                if constexpr (G::FOLD) {
-                    const uint32_t h = __shfl_sync(0xffffffffu, kh, kr + i * RPP);
-                    x = make_uint4(times(x.x, h), times(x.y, h), times(x.z, h), times(x.w, h));
-                    y = make_uint4(times(y.x, h), times(y.y, h), times(y.z, h), times(y.w, h));
+            for (uint32_t u = 0; u < G::SUB; u++) {
+#pragma unroll
+                for (uint32_t i = 0; i < KP; i++) {
+                    const uint4 w = kw[u][i];
+                    // codes 0, 2, 1, 3 of every four, as q's elements lie
+                    uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
+                    uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
+                    if constexpr (G::FOLD) {
+                        const uint32_t h = __shfl_sync(0xffffffffu, kh[u], kr + i * RPP);
+                        x = make_uint4(times(x.x, h), times(x.y, h), times(x.z, h), times(x.w, h));
+                        y = make_uint4(times(y.x, h), times(y.y, h), times(y.z, h), times(y.w, h));
+                    }
+                    // rows RPP apart: their places' swizzle is the same where RPP is 8, else it flips bit 2
+                    const uint32_t row = b * G::K_BYTES + (u * SP + i * RPP) * 128, flip = RPP == 4 && (i & 1) ? 64 : 0;
+                    sts128((to_k ^ flip) + row, x);
+                    sts128((to_k ^ flip ^ 16) + row, y);
                 }
-                // rows RPP apart: their places' swizzle is the same where RPP is 8, else it flips bit 2
-                const uint32_t row = b * G::K_BYTES + i * RPP * 128, flip = RPP == 4 && (i & 1) ? 64 : 0;
-                sts128((to_k ^ flip) + row, x);
-                sts128((to_k ^ flip ^ 16) + row, y);
+                if (t + 1 < tiles) load_k(t + 1, u);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&kfull[b]);
-            if (t + 1 < tiles) load_k(t + 1);
 
             if (use > 0) wait(&vempty[b], (use - 1) & 1);
-            if constexpr (!G::FOLD) {
-                if (lane < 16) {  // scales go with V: they are read until the weights are written
-                    sc[b * 2 * KT + 16 * cw + lane] = ks_now;
-                    sc[b * 2 * KT + KT + 16 * cw + lane] = vs_now;
-                }
-            }
 #pragma unroll
-            for (uint32_t v = 0; v < VP; v++) {
-                uint32_t h[4];
-                if constexpr (G::FOLD) {
-#pragma unroll
-                    for (uint32_t p = 0; p < 4; p++) h[p] = __shfl_sync(0xffffffffu, vh, 4 * (VP == 2 ? v : lane / DW) + p);
-                }
-                // elements d, d + 1, then d + 2, d + 3, by position pairs; group
-                // vg + 1's pieces lie beside group vg's: vg is even there
-                const uint32_t to = (to_v ^ (16 * v)) + b * G::V_BYTES;
-#pragma unroll
-                for (uint32_t e = 0; e < 4; e += 2) {
-                    uint32_t f[2][4];
-#pragma unroll
-                    for (uint32_t p = 0; p < 4; p++) {
-                        const uint32_t x = __byte_perm(vw[v][2 * p], vw[v][2 * p + 1], e == 0 ? 0x5410 : 0x7632);
-                        f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x);
-                        if constexpr (G::FOLD) f[0][p] = times(f[0][p], h[p]), f[1][p] = times(f[1][p], h[p]);
+            for (uint32_t u = 0; u < G::SUB; u++) {
+                if constexpr (!G::FOLD) {
+                    if (lane < 16) {  // scales go with V: they are read until the weights are written
+                        sc[b * 2 * KT + u * SP + 16 * cw + lane] = ks_now[u];
+                        sc[b * 2 * KT + KT + u * SP + 16 * cw + lane] = vs_now[u];
                     }
-                    sts128(to + e * (DW * 128), make_uint4(f[0][0], f[0][1], f[0][2], f[0][3]));
-                    sts128(to + (e + 1) * (DW * 128), make_uint4(f[1][0], f[1][1], f[1][2], f[1][3]));
                 }
+#pragma unroll
+                for (uint32_t v = 0; v < VP; v++) {
+                    uint32_t h[4];
+                    if constexpr (G::FOLD) {
+#pragma unroll
+                        for (uint32_t p = 0; p < 4; p++) h[p] = __shfl_sync(0xffffffffu, vh[u], 4 * (VP == 2 ? v : lane / DW) + p);
+                    }
+                    // elements d, d + 1, then d + 2, d + 3, by position pairs; group
+                    // vg + 1's pieces lie beside group vg's: vg is even there
+                    const uint32_t to = (to_v ^ (16 * v)) + b * G::V_BYTES + u * (SP / 64 * HD * 128);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e += 2) {
+                        uint32_t f[2][4];
+#pragma unroll
+                        for (uint32_t p = 0; p < 4; p++) {
+                            const uint32_t x = __byte_perm(vw[u][v][2 * p], vw[u][v][2 * p + 1], e == 0 ? 0x5410 : 0x7632);
+                            f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x);
+                            if constexpr (G::FOLD) f[0][p] = times(f[0][p], h[p]), f[1][p] = times(f[1][p], h[p]);
+                        }
+                        sts128(to + e * (DW * 128), make_uint4(f[0][0], f[0][1], f[0][2], f[0][3]));
+                        sts128(to + (e + 1) * (DW * 128), make_uint4(f[1][0], f[1][1], f[1][2], f[1][3]));
+                    }
+                }
+                if (t + 1 < tiles) load_v(t + 1, u);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&vfull[b]);
-            if (t + 1 < tiles) load_v(t + 1);
         }
     } else {
         // ---------------------------------------------------- one row tile
+        if constexpr (G::OREG) tc5::setmaxnreg_inc<kChunkRegsRow>();
         const uint32_t w = warp / 4, th = tid % 128, row = w * 128 + th;
         if (w < users) {
             const bool on = row < live;
@@ -939,7 +962,7 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                 tc5::fence_after();
                 if (tc5::elect()) {
                     const uint64_t vd = v_desc + b * (G::V_BYTES / 16);
-                    const bool more = t > 0;
+                    const bool more = !G::OREG && t > 0;
 #pragma unroll
                     for (uint32_t k = 0; k < KT / 16; k++) {
                         const uint32_t at = k / 4 * (HD * 128 / 16) + 2 * (k % 4);
@@ -1009,6 +1032,21 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                 tc5::st8(scol + lanes + 16 * c, wh);
                 if constexpr (G::WPAIR) tc5::st8(scol + lanes + 16 * c + 8, wl);
             };
+            float o[G::OREG ? HD : 1], alpha = 1.0f;  // OREG: the outputs, and what they take when tile t's are added
+#pragma unroll
+            for (uint32_t i = 0; i < (G::OREG ? HD : 1); i++) o[i] = 0.0f;
+            auto add_o = [&](uint32_t t) {
+                wait(&o_done[w], t & 1);
+                tc5::fence_after();
+#pragma unroll
+                for (uint32_t c = 0; c < (G::OREG ? HD / 16 : 0); c++) {
+                    float y[16];
+                    tc5::ld16(ocol + lanes + 16 * c, y);
+                    tc5::wait_ld();
+#pragma unroll
+                    for (uint32_t i = 0; i < 16; i++) o[16 * c + i] = fmaf(o[16 * c + i], alpha, y[i]);
+                }
+            };
             // One tile: the scores are read twice, for their maximum and for the
             // weights, so that few registers hold them; the next columns are on
             // their way from TMEM while these are worked on.
@@ -1027,12 +1065,18 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                     scaled(ks, c + 1, y);
                     top = largest(masked, c + 1, y, top, left);
                 }
+                if constexpr (G::OREG) {
+                    if (t > 0) {
+                        tc5::wait_ld();
+                        add_o(t - 1);
+                    }
+                }
                 top *= cf;
                 const bool up = top > mx + kSlack;
-                const float alpha = up ? ex2(mx - top) : 1.0f;
+                alpha = up ? ex2(mx - top) : 1.0f;
                 l *= alpha;
                 mx = up ? top : mx;
-                if (t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum
+                if (!G::OREG && t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum
                     tc5::wait_ld();
                     wait(&o_done[w], (t - 1) & 1);
                     tc5::fence_after();
@@ -1075,8 +1119,15 @@ __global__ void __launch_bounds__(512, 1) k_kv8_chunk(const Kv8AttendArgs a) {
                     if (t + 1 < tiles) issue_s(t + 1);
                 }
             }
-            wait(&o_done[w], (tiles - 1) & 1);
-            tc5::fence_after();
+            if constexpr (G::OREG) {  // their sums back where the last tile's were
+                add_o(tiles - 1);
+#pragma unroll
+                for (uint32_t c = 0; c < HD / 8; c++) tc5::st8(ocol + lanes + 8 * c, reinterpret_cast<const uint32_t*>(o + (G::OREG ? 8 * c : 0)));
+                tc5::wait_st();
+            } else {
+                wait(&o_done[w], (tiles - 1) & 1);
+                tc5::fence_after();
+            }
             // what a row's outputs are divided by goes through shared memory: the
             // registers of this loop stay its own (rows that see nothing: sums of 0)
             float vunit;
@@ -1153,6 +1204,11 @@ cudaError_t set_limits() {
         e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 2>::RING);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_kv8_chunk<HD, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkGeom<HD, DT>::BYTES);
+    // what setmaxnreg deals out has to be there
+    cudaFuncAttributes at{};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, k_kv8_chunk<HD, DT>);
+    if (e == cudaSuccess && ChunkGeom<HD, DT>::OREG && at.numRegs * 3 < 2 * kChunkRegsRow + kChunkRegsCode)
+        e = cudaErrorInvalidConfiguration;
     return e;
 }
 

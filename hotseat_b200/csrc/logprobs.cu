@@ -1,5 +1,25 @@
 // Scores of logit rows: log probabilities of given tokens, entropy, rank and
-// the top alternatives.
+// the top alternatives, in one pass over the logits.
+//
+// A row is taken by a cluster of up to 8 CTAs, each a contiguous share that
+// its 512 threads hold in registers, so the logits are read once: the
+// maximum, then sum exp(x - m) and sum exp(x - m)(x - m) (for the entropy
+// ln l - t / l), the tokens before the given one, and the top candidates all
+// come from the registers. The CTAs' results meet in distributed shared
+// memory; nothing is kept in global memory between them, so calls on several
+// streams share nothing.
+//
+// Top candidates: the order's key of a token is unique, so the `top`-th
+// largest of the largest keys of 32 or 64 thread groups is a bound that all of
+// a CTA's top tokens reach, and few others: these are collected and each
+// placed by counting the larger ones. Where more tokens reach it than there is
+// room for (logits in order, say), the bound is taken from the threads' own
+// largest keys, which leaves at most 64 x 40. The cluster's first CTA merges
+// the CTAs' lists the same way.
+//
+// A row that is longer than a cluster holds (163,840 logits) goes through the
+// registers in strips, their results joined as the CTAs' are.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -10,102 +30,366 @@
 #include "kernels.h"
 #include "kv_region.h"
 
+namespace cg = cooperative_groups;
+
 namespace hs {
 namespace {
 
+constexpr uint32_t kThreads = 512, kPer = 40;       // logits a thread holds
+constexpr uint32_t kStrip = kThreads * kPer;        // logits a CTA holds
+constexpr uint32_t kCluster = 8;
+constexpr uint32_t kCand = kLogprobTop * kPer + kLogprobTop;  // candidates at most, and the strips' so far
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 template <int DT>
 __device__ __forceinline__ float logit(const void* p, uint64_t e) {
-    if constexpr (DT == HS_F32) return static_cast<const float*>(p)[e];
+    if constexpr (DT == HS_F32) return __ldg(static_cast<const float*>(p) + e);
     else if constexpr (DT == HS_F16) return __half2float(static_cast<const __half*>(p)[e]);
     else return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[e]);
 }
 
-// A key that is larger for a token that comes earlier in the order (logit
-// descending, NaN first, -0 equal to 0; id ascending).
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t id) {
+// The order of logits as unsigned numbers (NaN first, -0 equal to 0), and the
+// key of a token: larger for one that comes earlier (logit descending, id
+// ascending). Never 0 for a token.
+__device__ __forceinline__ uint32_t order(float x) {
     uint32_t b = __float_as_uint(__fadd_rn(x, 0.0f));
     b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    if (isnan(x)) b = 0xffffffffu;
-    return ((uint64_t)b << 32) | (0xffffffffu - id);
+    return isnan(x) ? 0xffffffffu : b;
+}
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t id) { return ((uint64_t)order(x) << 32) | (0xffffffffu - id); }
+__device__ __forceinline__ uint32_t key_id(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
+
+// sum exp(x - m) and sum exp(x - m)(x - m) of some logits with maximum m, and
+// how many come before the given token.
+struct Sums {
+    double l = 0.0, t = 0.0;
+    float m = -INFINITY;
+    uint32_t before = 0;
+};
+// Two disjoint sets of logits as one. A NaN in either stays.
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    r.before = a.before + b.before;
+    auto add = [&](const Sums& x) {
+        if (isnan(x.l) || isnan(x.t)) {
+            r.l = r.t = __longlong_as_double(0x7ff8000000000000ll);
+        } else if (x.l != 0.0) {
+            const double d = (double)x.m - (double)r.m, w = exp(d);
+            r.l += x.l * w;
+            r.t += (x.t + x.l * d) * w;
+        }
+    };
+    add(a);
+    add(b);
+    return r;
 }
 
-constexpr uint32_t kThreads = 512;
+struct Shared {
+    double l[16], t[16];
+    float m[16];
+    uint32_t before[16], n_cand;
+    uint64_t bound;
+    uint64_t group[64];            // largest key of a thread group
+    uint64_t best[kThreads];       // ... of a thread (the second way)
+    uint64_t cand[kCand];
+    uint64_t all[kCluster * kLogprobTop];
+    // what the other CTAs of the row read: the top tokens in order (0: none), the sums
+    uint64_t top[kLogprobTop];
+    Sums sums;
+};
+
+// Logit i = (j * 512 + tid) * V + e of a strip is this thread's number V j + e.
+template <int V>
+__device__ __forceinline__ uint32_t place(uint32_t k) {
+    return ((k / V) * kThreads + threadIdx.x) * V + k % V;
+}
+
+template <int DT, int V>
+__global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, uint32_t share) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared& s = *reinterpret_cast<Shared*>(smem);
+    constexpr uint32_t EB = DT == HS_F32 ? 4 : 2;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    cg::cluster_group cl = cg::this_cluster();
+    const uint32_t rank = blockIdx.x, ctas = gridDim.x;
+    const uint64_t r = blockIdx.y + (uint64_t)blockIdx.z * gridDim.y;
+    if (r >= a.rows) return;  // the whole cluster
+    const uint8_t* row = static_cast<const uint8_t*>(a.logits) + r * a.row_stride * EB;
+    const uint32_t id = a.ids ? __ldg(a.ids + r) : 0xffffffffu;
+    const float xt = id < a.vocab ? logit<DT>(row, id) : __int_as_float(0x7fc00000);
+    const uint32_t begin = min(rank * share, a.vocab), end = min(begin + share, a.vocab);
+    Sums sums;
+    if (tid < kLogprobTop) s.top[tid] = 0;
+
+    for (uint32_t from = begin; from < end; from += kStrip) {
+        const uint32_t n = min(kStrip, end - from);
+        const uint8_t* mine = row + (uint64_t)from * EB;
+        // the strip, -inf behind its end
+        float x[kPer];
+#pragma unroll
+        for (uint32_t j = 0; j < kPer / V; j++) {
+            const uint32_t i = (j * kThreads + tid) * V;
+            if (V > 1 && i + V <= n) {
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(mine + (uint64_t)i * EB));
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    if constexpr (DT == HS_F32) {
+                        x[V * j + e % V] = __uint_as_float(u[e]);
+                    } else if constexpr (DT == HS_F16) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+                        x[V * j + 2 * e % V] = f.x, x[V * j + (2 * e + 1) % V] = f.y;
+                    } else {
+                        x[V * j + 2 * e % V] = __uint_as_float(u[e] << 16), x[V * j + (2 * e + 1) % V] = __uint_as_float(u[e] & 0xffff0000u);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < V; e++) x[V * j + e] = i + e < n ? logit<DT>(mine, i + e) : -INFINITY;
+            }
+        }
+        // the strip's maximum (NaN skipped: it shows in the sums)
+        float m = -INFINITY;
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; k++) m = fmaxf(m, x[k]);
+        const float mine_top = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) s.m[warp] = m;
+        if (tid == 0) s.n_cand = 0, s.bound = 0;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < 16; w++) m = fmaxf(m, s.m[w]);
+
+        // Sums over eight logits in f32, over more in f64. A logit 200 below the
+        // maximum has no weight, and its distance is cut there: 0 times -inf is not.
+        double l = 0.0, t = 0.0;
+        const float shift = m == -INFINITY ? 0.0f : -m;
+        const uint64_t shift2 = pack2(shift, shift), log2e2 = pack2(kLog2e, kLog2e);
+#pragma unroll
+        for (uint32_t k = 0; k < kPer; k += 8) {
+            uint64_t lp[4], tp[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint64_t d2 = add2(pack2(x[k + 2 * e], x[k + 2 * e + 1]), shift2);
+                float d0, d1, y0, y1;
+                unpack2(d2, &d0, &d1);
+                unpack2(mul2(d2, log2e2), &y0, &y1);
+                lp[e] = pack2(ex2(y0), ex2(y1));
+                tp[e] = mul2(lp[e], pack2(fmaxf(d0, -200.0f), fmaxf(d1, -200.0f)));
+            }
+            const uint64_t ls = add2(add2(lp[0], lp[1]), add2(lp[2], lp[3])), ts = add2(add2(tp[0], tp[1]), add2(tp[2], tp[3]));
+            float l0, l1, t0, t1;
+            unpack2(ls, &l0, &l1);
+            unpack2(ts, &t0, &t1);
+            l += (double)(l0 + l1), t += (double)(t0 + t1);
+        }
+        uint32_t before = 0;
+        if (a.rank && id < a.vocab) {
+            if (isnan(xt)) {  // before it: NaNs of lower ids
+#pragma unroll
+                for (uint32_t k = 0; k < kPer; k++) before += isnan(x[k]) && from + place<V>(k) < id ? 1 : 0;
+            } else {
+                // greater or NaN, or equal with a lower id: not below, by ids, a
+                // bound of xt or of the number just under it (none under -inf: NaN)
+                float under = xt == 0.0f ? __int_as_float(0x80000001u) : __int_as_float(__float_as_int(xt) + (xt < 0.0f ? 1 : -1));
+                if (xt == -INFINITY) under = __int_as_float(0x7fc00000);
+#pragma unroll
+                for (uint32_t k = 0; k < kPer; k++) {
+                    const uint32_t p = place<V>(k);
+                    before += p < n && !(x[k] <= (from + p < id ? under : xt)) ? 1 : 0;
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        if (lane == 0) s.l[warp] = l, s.t[warp] = t, s.before[warp] = before;
+
+        if (a.top) {
+            // the thread's largest key: a NaN, else its largest logit, the first of equal ones
+            uint32_t at = kPer;
+            bool nan = false;
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; i++) {
+                const uint32_t k = kPer - 1 - i;
+                if (!(x[k] < mine_top)) at = k;
+                nan |= isnan(x[k]);
+            }
+            uint64_t best = 0;
+            if (nan || mine_top == -INFINITY) {
+#pragma unroll
+                for (uint32_t k = 0; k < kPer; k++) {
+                    const uint64_t key = order_key(x[k], from + place<V>(k));
+                    if (place<V>(k) < n && key > best) best = key;
+                }
+            } else {
+                best = order_key(mine_top, from + place<V>(at));
+            }
+            // groups of 16 threads, of 8 for more than 16 tokens; the bound is the
+            // key that top - 1 of theirs are above (0 if fewer hold any)
+            const uint32_t size = a.top <= 16 ? 16 : 8, groups = kThreads / size;
+            uint64_t g = best;
+            for (uint32_t o = size / 2; o > 0; o >>= 1) {
+                const uint64_t other = __shfl_xor_sync(0xffffffffu, g, o);
+                g = other > g ? other : g;
+            }
+            if (tid % size == 0) s.group[tid / size] = g;
+            __syncthreads();
+            if (tid < groups) {
+                const uint64_t key = s.group[tid];
+                uint32_t above = 0;
+#pragma unroll 16
+                for (uint32_t i = 0; i < groups; i++) above += s.group[i] > key ? 1 : 0;
+                if (key && above == a.top - 1) s.bound = key;
+            }
+            if (tid < a.top && s.top[tid]) {  // the strips' so far stand with this one's
+                s.cand[atomicAdd(&s.n_cand, 1u)] = s.top[tid];
+                s.top[tid] = 0;
+            }
+            __syncthreads();
+            const uint32_t held = s.n_cand;
+            auto collect = [&](uint64_t bound) {
+                if (best && best >= bound) {
+                    const uint32_t b = (uint32_t)(bound >> 32);
+                    // the bound's logit: nothing below it is a candidate
+                    const float low = bound == 0 || b == 0xffffffffu ? -INFINITY : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+#pragma unroll
+                    for (uint32_t k = 0; k < kPer; k++)
+                        if (!(x[k] < low)) {
+                            const uint64_t key = order_key(x[k], from + place<V>(k));
+                            if (place<V>(k) < n && key >= bound) {
+                                const uint32_t c = atomicAdd(&s.n_cand, 1u);
+                                if (c < kCand) s.cand[c] = key;
+                            }
+                        }
+                }
+            };
+            collect(s.bound);
+            __syncthreads();
+            if (s.n_cand > kCand) {  // the same for every thread
+                s.best[tid] = best;
+                __syncthreads();
+                if (tid == 0) s.n_cand = held, s.bound = 0;
+                __syncthreads();
+                uint32_t above = 0;
+                for (uint32_t i = 0; i < kThreads; i++) above += s.best[i] > best ? 1 : 0;
+                if (best && above == a.top - 1) s.bound = best;
+                __syncthreads();
+                collect(s.bound);
+                __syncthreads();
+            }
+            const uint32_t nc = s.n_cand;
+            for (uint32_t i = tid; i < nc; i += kThreads) {
+                const uint64_t key = s.cand[i];
+                uint32_t above = 0;
+                for (uint32_t j = 0; j < nc; j++) above += s.cand[j] > key ? 1 : 0;
+                if (above < a.top) s.top[above] = key;
+            }
+        }
+        __syncthreads();
+        Sums strip;
+        strip.m = m;
+#pragma unroll
+        for (int w = 0; w < 16; w++) strip.l += s.l[w], strip.t += s.t[w], strip.before += s.before[w];
+        if (m == -INFINITY && !isnan(strip.l)) strip.l = strip.t = 0.0;
+        sums = from == begin ? strip : join(sums, strip);
+        __syncthreads();  // the arrays are free for the next strip
+    }
+    if (tid == 0) s.sums = sums;
+    cl.sync();
+    const uint32_t nk = ctas * a.top;
+    if (rank == 0) {  // the CTAs' results, then they may leave
+        if (tid < ctas) sums = *cl.map_shared_rank(&s.sums, tid);
+        for (uint32_t i = tid; i < nk; i += kThreads) s.all[i] = cl.map_shared_rank(s.top, i / a.top)[i % a.top];
+    }
+    cl.sync();
+    if (rank != 0) return;
+    if (warp == 0) {
+        for (uint32_t o = 1; o < ctas; o <<= 1) {  // lanes 0 .. ctas - 1, a power of two
+            Sums other;
+            other.l = __shfl_xor_sync(0xffffffffu, sums.l, o);
+            other.t = __shfl_xor_sync(0xffffffffu, sums.t, o);
+            other.m = __shfl_xor_sync(0xffffffffu, sums.m, o);
+            other.before = __shfl_xor_sync(0xffffffffu, sums.before, o);
+            sums = lane & o ? join(other, sums) : join(sums, other);
+        }
+        // nothing but -inf, or +inf: no distribution
+        if (sums.m == -INFINITY || sums.m == INFINITY) sums.l = sums.t = __longlong_as_double(0x7ff8000000000000ll);
+        const double lz = log(sums.l);
+        if (lane == 0) {
+            s.m[0] = sums.m;
+            s.m[1] = (float)lz;
+            if (a.logp) a.logp[r] = (xt - sums.m) - (float)lz;
+            if (a.entropy) a.entropy[r] = (float)(lz - sums.t / sums.l);
+            if (a.rank) a.rank[r] = id < a.vocab ? sums.before : 0xffffffffu;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < nk; i += kThreads) {
+        const uint64_t key = s.all[i];
+        if (!key) continue;
+        uint32_t above = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < nk; j++) above += s.all[j] > key ? 1 : 0;
+        if (above < a.top) {
+            const uint32_t tok = key_id(key);
+            if (a.top_ids) a.top_ids[r * a.top + above] = tok;
+            if (a.top_logp) a.top_logp[r * a.top + above] = (logit<DT>(row, tok) - s.m[0]) - s.m[1];
+        }
+    }
+}
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) k_logprobs_simple(const LogprobArgs a) {
-    __shared__ float fa[16];
-    __shared__ double da[16], db[16];
-    __shared__ uint32_t ua[16];
-    __shared__ uint64_t ka[16];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint64_t r = blockIdx.x;
-    const uint8_t* row = static_cast<const uint8_t*>(a.logits) + r * a.row_stride * (DT == HS_F32 ? 4 : 2);
-    const uint32_t id = a.ids ? a.ids[r] : 0xffffffffu;
-    const float xt = id < a.vocab ? logit<DT>(row, id) : __int_as_float(0x7fffffff);
-    const uint64_t kt = order_key(xt, id);
-    float m = -INFINITY;
-    for (uint32_t i = tid; i < a.vocab; i += kThreads) m = fmaxf(m, logit<DT>(row, i));
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) fa[warp] = m;
-    __syncthreads();
-    for (int w = 0; w < 16; w++) m = fmaxf(m, fa[w]);
-    __syncthreads();
-    double l = 0.0, t = 0.0;
-    uint32_t before = 0;
-    for (uint32_t i = tid; i < a.vocab; i += kThreads) {
-        const float x = logit<DT>(row, i), d = x - m, e = expf(d);
-        l += e;
-        if (e != 0.0f) t += (double)e * d;
-        before += order_key(x, i) > kt;
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-        l += __shfl_xor_sync(0xffffffffu, l, o);
-        t += __shfl_xor_sync(0xffffffffu, t, o);
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-    }
-    if (lane == 0) da[warp] = l, db[warp] = t, ua[warp] = before;
-    __syncthreads();
-    l = t = 0.0;
-    before = 0;
-    for (int w = 0; w < 16; w++) l += da[w], t += db[w], before += ua[w];
-    const float lz = (float)log(l);
-    if (tid == 0) {
-        if (a.logp) a.logp[r] = (xt - m) - lz;
-        if (a.entropy) a.entropy[r] = (float)(log(l) - t / l);
-        if (a.rank) a.rank[r] = id < a.vocab ? before : 0xffffffffu;
-    }
-    uint64_t last = ~0ull;
-    for (uint32_t j = 0; j < a.top; j++) {
-        uint64_t best = 0;
-        for (uint32_t i = tid; i < a.vocab; i += kThreads) {
-            const uint64_t k = order_key(logit<DT>(row, i), i);
-            if ((j == 0 || k < last) && k > best) best = k;
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
-            best = k > best ? k : best;
-        }
-        if (lane == 0) ka[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < 16; w++) best = ka[w] > best ? ka[w] : best;
-        __syncthreads();
-        last = best;
-        if (tid == 0) {
-            const uint32_t i = 0xffffffffu - (uint32_t)best;
-            if (a.top_ids) a.top_ids[r * a.top + j] = i;
-            if (a.top_logp) a.top_logp[r * a.top + j] = (logit<DT>(row, i) - m) - lz;
-        }
-    }
+cudaError_t launch_dt(const LogprobArgs& a, cudaStream_t st) {
+    // Shares of a multiple of 8 logits, so that they start as aligned as the row
+    // does; a short row's are 4,096 logits at least.
+    constexpr int V = DT == HS_F32 ? 4 : 8;
+    uint32_t ctas = 1;
+    while (ctas < kCluster && ctas * 4096u < a.vocab) ctas *= 2;
+    const uint32_t share = ((a.vocab + ctas - 1) / ctas + 7) / 8 * 8;
+    const uint64_t bytes = DT == HS_F32 ? 4 : 2;
+    const bool vec = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride * bytes % 16 == 0;
+    cudaLaunchConfig_t cfg = {};
+    const uint32_t ry = a.rows < 65535 ? a.rows : 65535;
+    cfg.gridDim = dim3(ctas, ry, (a.rows + ry - 1) / ry);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.stream = st;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return vec ? cudaLaunchKernelEx(&cfg, k_logprobs<DT, V>, a, share) : cudaLaunchKernelEx(&cfg, k_logprobs<DT, 1>, a, share);
 }
 
 }  // namespace
 
 cudaError_t launch_logprobs(const LogprobArgs& a, cudaStream_t st) {
     if (!a.rows) return cudaSuccess;
-    if (a.dtype == HS_F32) k_logprobs_simple<HS_F32><<<a.rows, kThreads, 0, st>>>(a);
-    else if (a.dtype == HS_F16) k_logprobs_simple<HS_F16><<<a.rows, kThreads, 0, st>>>(a);
-    else k_logprobs_simple<HS_BF16><<<a.rows, kThreads, 0, st>>>(a);
-    return cudaGetLastError();
+    return a.dtype == HS_F32 ? launch_dt<HS_F32>(a, st) : a.dtype == HS_F16 ? launch_dt<HS_F16>(a, st) : launch_dt<HS_BF16>(a, st);
 }
 
 int check_logprobs(uint32_t rows, uint32_t vocab, const void* ids, uint32_t top, const void* logp, const void* rank,

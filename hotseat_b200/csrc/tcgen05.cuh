@@ -101,5 +101,15 @@ __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
         : "memory");
 }
 
+// Registers a thread of the (converged) warpgroup, up or down.
+template <uint32_t N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <uint32_t N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 }  // namespace tc5
 }  // namespace hs
