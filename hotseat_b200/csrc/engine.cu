@@ -1990,6 +1990,12 @@ struct hs_batch {
     float* sc_global = nullptr;    // attention scores for long contexts [cap_slots][nh][max_ctx]
     float* att_part = nullptr;     // split-KV attention partials [cap_slots][nkv][max_splits][record]
     uint32_t* att_cnt = nullptr;   // [cap_slots][nkv]
+    // 8-bit regions (block8: their scale block, 0 for f32 ones), at their first
+    // use: rows of q, k, v and of the attention, positions, its workspace
+    uint32_t block8 = 0;
+    float *q8 = nullptr, *k8 = nullptr, *v8 = nullptr, *o8 = nullptr, *part8 = nullptr;
+    uint32_t *pos8 = nullptr, *start8 = nullptr, *counters8 = nullptr;
+    hs::Kv8Plan plan8;
     float* pf_part = nullptr;      // prefill segment records [cap_slots][nkv][pf_nseg][record], at first prefill
     uint64_t* trace = nullptr;     // launch timeline (HS_TRACE=1 at creation): 8 u64 per launch
     uint64_t* trace_init = nullptr;
@@ -2012,7 +2018,8 @@ struct hs_batch {
                         (void*)hb_hi, (void*)hb_lo, (void*)ctl, (void*)tokens, (void*)tok_tab, (void*)kv_tab,
                         (void*)dirty_tab, (void*)track_tab, (void*)cand, (void*)argbuf, (void*)err,
                         (void*)sc_global, (void*)att_part, (void*)att_cnt, (void*)sort_cand, (void*)wkeys,
-                        (void*)wps, (void*)nll, (void*)nll_next, (void*)scores, (void*)pf_part})
+                        (void*)wps, (void*)nll, (void*)nll_next, (void*)scores, (void*)pf_part, (void*)q8, (void*)k8, (void*)v8,
+                        (void*)o8, (void*)part8, (void*)pos8, (void*)start8, (void*)counters8})
             cudaFree(p);
     }
 };
@@ -2062,7 +2069,68 @@ int batch_gemm(hs_batch* b, const TcGemmPlan& p, const uint16_t* a_hi, const uin
     return HS_OK;
 }
 
-// One batched forward for slots [0, n): 7 launches per layer + final norm + LM head.
+// Buffers and limits of 8-bit regions' attention, before any capture.
+int batch_ensure_kv8(hs_batch* b) {
+    if (b->q8) return HS_OK;
+    const hs_config& c = b->m->cfg;
+    const uint64_t C = b->cap_slots;
+    HS_CUDA_TRY(kv8_attend_set_smem_limits());
+    b->plan8 = kv8_plan(model_kv_spec(b->m, 0), c.n_heads, b->cap_slots);
+    auto alloc = [&](auto** p, uint64_t count) -> int {
+        cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), std::max<uint64_t>(count, 1) * 4);
+        if (e != cudaSuccess) return fail(HS_E_NOMEM, std::string("cudaMalloc: ") + cudaGetErrorString(e));
+        return HS_OK;
+    };
+    float* q8 = nullptr;  // set last: the sign that all are there
+    int rc;
+    if ((rc = alloc(&b->k8, C * c.n_kv_heads * c.head_dim)) || (rc = alloc(&b->v8, C * c.n_kv_heads * c.head_dim)) ||
+        (rc = alloc(&b->o8, C * c.n_heads * c.head_dim)) || (rc = alloc(&b->pos8, C)) || (rc = alloc(&b->start8, 2)) ||
+        (rc = alloc(&b->part8, b->plan8.part_floats)) || (rc = alloc(&b->counters8, b->plan8.counters)) ||
+        (rc = alloc(&q8, C * c.n_heads * c.head_dim)))
+        return rc;
+    b->q8 = q8;
+    HS_CUDA_TRY(cudaMemsetAsync(b->counters8, 0, std::max<uint64_t>(b->plan8.counters, 1) * 4, b->st));
+    return HS_OK;
+}
+
+// Attention of one layer over 8-bit regions in four launches: q, k, v rows, the
+// append, the attention (single rows, or a prompt's as one chunk), f16 pairs.
+int batch_attend_kv8(hs_batch* b, const SplitAttnArgs& sa, uint32_t n, bool prefill, uint32_t* launches) {
+    const hs_config& c = b->m->cfg;
+    const uint32_t hd = c.head_dim;
+    const hs_kv_spec spec = model_kv_spec(b->m, b->layout);
+    Kv8AttendArgs a;
+    a.kv = kv8_view(spec, b->block8, sa.layer);
+    a.kv.base = b->kv_tab;
+    a.kv.dirty = b->dirty_tab;
+    a.kv.tracking = b->track_tab;
+    a.kv.n_slots = prefill ? 1 : n;
+    a.kv.page_shift = b->page_shift;
+    a.rows.n_rows = n;
+    a.rows.n_slots = a.kv.n_slots;
+    a.rows.row_start = prefill ? b->start8 : nullptr;
+    a.rows.pos = b->pos8;
+    a.rows.err = b->err;
+    a.q = Kv8Mat{b->q8, (uint64_t)c.n_heads * hd, hd, HS_F32};
+    a.out = Kv8Mat{b->o8, (uint64_t)c.n_heads * hd, hd, HS_F32};
+    a.q_vec = a.out_vec = true;
+    a.nh = c.n_heads;
+    a.scale = 1.0f / std::sqrt((float)hd);
+    kv8_use_plan(&a, b->plan8);
+    a.part = b->part8;
+    a.counters = b->counters8;
+    const Kv8Mat k{b->k8, (uint64_t)c.n_kv_heads * hd, hd, HS_F32}, v{b->v8, (uint64_t)c.n_kv_heads * hd, hd, HS_F32};
+    cudaError_t e = launch_kv8_qkv_rows(hd, sa, n, b->q8, b->k8, b->v8, b->pos8, b->start8, b->st);
+    if (e == cudaSuccess) e = launch_kv8_append(hd, a.kv, a.rows, k, v, b->st);
+    if (e == cudaSuccess) e = launch_kv8_attend(hd, a, b->st);
+    if (e == cudaSuccess) e = launch_kv8_to_pairs(b->o8, (uint64_t)n * c.n_heads * hd, b->att_hi, b->att_lo, b->st);
+    if (e != cudaSuccess) return fail(HS_E_CUDA, std::string("8-bit attention launch: ") + cudaGetErrorString(e));
+    *launches += 3;  // the caller counts the last
+    return HS_OK;
+}
+
+// One batched forward for slots [0, n): 7 launches per layer (10 over 8-bit
+// regions) + final norm + LM head.
 int batch_enqueue_forward(hs_batch* b, uint32_t n, uint32_t* launches, bool prefill) {
     const hs_model* m = b->m;
     const hs_config& c = m->cfg;
@@ -2133,7 +2201,10 @@ int batch_enqueue_forward(hs_batch* b, uint32_t n, uint32_t* launches, bool pref
             sa.tensor_cores = m->numeric == HS_NUMERIC_TC ? 1u : 0u;
             sa.trace = b->trace;
             sa.trace_slot = *launches;
-            if (prefill) {
+            if (b->block8) {
+                if ((rc = batch_attend_kv8(b, sa, n, prefill, launches))) return rc;
+                e = cudaSuccess;
+            } else if (prefill) {
                 // tokens of one sequence: every k, v appended before any attends
                 sa.mode = ATTN_APPEND_ONLY;
                 e = m->pf_qblock ? launch_prefill_append(hd, sa, n, b->st) : launch_attn_split(hd, sa, n, b->st);
@@ -2142,7 +2213,9 @@ int batch_enqueue_forward(hs_batch* b, uint32_t n, uint32_t* launches, bool pref
                 sa.mode = ATTN_ATTEND_ONLY;
                 sa.trace_slot = *launches;
             }
-            if (prefill && m->pf_qblock) {
+            if (b->block8) {
+                // done, all but the count of the last launch
+            } else if (prefill && m->pf_qblock) {
                 // query blocks over fixed segments, then the segments' merge
                 sa.partials = b->pf_part;
                 sa.max_splits = m->pf_nseg;
@@ -2195,7 +2268,7 @@ SampleArgs batch_sample_args(hs_batch* b, uint32_t n, uint32_t kmax) {
 int batch_graph(hs_batch* b, uint32_t n, uint32_t kmax, cudaGraphExec_t* out, uint32_t* launches,
                 bool prefill = false) {
     const uint64_t key = (uint64_t)n | (uint64_t)kmax << 16 | (uint64_t)b->layout << 32 | (uint64_t)b->page_shift << 40 |
-                         (uint64_t)prefill << 48;
+                         (uint64_t)prefill << 48 | (uint64_t)b->block8 << 52;
     auto it = b->graphs.find(key);
     if (it != b->graphs.end()) {
         *out = it->second.first;
@@ -2236,11 +2309,17 @@ int batch_kv_tables(hs_batch* b, hs_kv* const* kvs, uint32_t n, bool same_sequen
         if (!kvs[i]) return fail(HS_E_ARG, "null KV region");
         int rc = check_kv(m, kvs[i]);
         if (rc) return rc;
-        if (kvs[i]->spec.layout != kvs[0]->spec.layout || kvs[i]->page_shift != kvs[0]->page_shift)
-            return fail(HS_E_ARG, "KV regions of one batch must share layout and page size");
+        if (kvs[i]->spec.layout != kvs[0]->spec.layout || kvs[i]->page_shift != kvs[0]->page_shift ||
+            kvs[i]->block8 != kvs[0]->block8)
+            return fail(HS_E_ARG, "KV regions of one batch must share layout, page size and format");
         for (uint32_t j = 0; j < i && !same_sequence; j++)
             if (kvs[j] == kvs[i]) return fail(HS_E_ARG, "a KV region appears twice in one batch");
     }
+    if (kvs[0]->block8) {
+        int rc = batch_ensure_kv8(b);
+        if (rc) return rc;
+    }
+    b->block8 = kvs[0]->block8;
     b->layout = kvs[0]->spec.layout;
     b->page_shift = kvs[0]->page_shift;
     void** h = b->tab_h;
@@ -2260,7 +2339,7 @@ int batch_sync(hs_batch* b, uint32_t n) {
     HS_CUDA_TRY(cudaMemcpyAsync(b->ctl_h, b->ctl, (size_t)n * sizeof(DevCtl), cudaMemcpyDeviceToHost, b->st));
     HS_CUDA_TRY(cudaMemcpyAsync(&b->err_h, b->err, 4, cudaMemcpyDeviceToHost, b->st));
     HS_CUDA_TRY(cudaStreamSynchronize(b->st));
-    if (b->err_h) return fail(HS_E_CUDA, "tensor-core GEMM reported a bounded-wait timeout");
+    if (b->err_h) return fail(HS_E_CUDA, "tensor-core GEMM or attention reported a bounded-wait timeout");
     for (uint32_t i = 0; i < n; i++) {
         int rc = ctl_err(b->ctl_h[i].err);
         if (rc) return fail(rc, "sequence " + std::to_string(i) + ": " + hs_last_error());
@@ -2322,7 +2401,7 @@ int hs_batch_new(const hs_model* m, uint32_t max_seqs, hs_batch** out) {
     HS_CUDA_TRY(cudaMallocHost(&b->tab_h, (size_t)3 * C * sizeof(void*)));
     const char* tenv = getenv("HS_TRACE");
     if (tenv && tenv[0] == '1') {
-        b->trace_slots = c.n_layers * 9 + 5;  // prefill: 9 launches a layer; decode: 7 + norm, head, sampler
+        b->trace_slots = c.n_layers * 10 + 5;  // prefill: 9 launches a layer (8-bit regions: 10); decode: 7 + norm, head, sampler
         HS_CUDA_TRY(cudaMalloc(&b->trace, (size_t)b->trace_slots * 64));
         HS_CUDA_TRY(cudaMallocHost(&b->trace_init, (size_t)b->trace_slots * 64));
         for (uint32_t i = 0; i < b->trace_slots; i++) {

@@ -134,6 +134,42 @@ struct Kv8AttendArgs {
 cudaError_t kv8_attend_set_smem_limits();
 cudaError_t launch_kv8_attend(uint32_t hd, const Kv8AttendArgs& a, cudaStream_t st);
 
+// The splits and workspace of single rows for n slots: what Kv8AttendArgs needs.
+struct Kv8Plan {
+    uint32_t group = 0, chunks = 0, max_splits = 0, cluster = 1, max_clusters = 0;
+    uint64_t part_floats = 0, counters = 0;  // 0: none needed
+};
+inline Kv8Plan kv8_plan(const hs_kv_spec& s, uint32_t nh, uint32_t n) {
+    Kv8Plan p;
+    p.group = nh / s.n_kv_heads;
+    const uint32_t nc = kv8_single_cols(p.group), least = kv8_min_split(s.head_dim);
+    p.chunks = (p.group + nc - 1) / nc;
+    const uint64_t items = (uint64_t)n * s.n_kv_heads * p.chunks;
+    const uint32_t splits = (s.max_ctx + least - 1) / least;
+    p.max_splits = splits < kv8_max_splits(s.n_kv_heads) ? splits : kv8_max_splits(s.n_kv_heads);
+    while (p.cluster < 8 && p.cluster < p.max_splits) p.cluster *= 2;
+    p.max_clusters = (p.max_splits + p.cluster - 1) / p.cluster;
+    if (p.max_clusters > 1) {
+        p.part_floats = items * p.max_clusters * kv8_record(s.head_dim, nc);
+        p.counters = items * 8;
+    }
+    return p;
+}
+inline void kv8_use_plan(Kv8AttendArgs* a, const Kv8Plan& p) {
+    a->group = p.group;
+    a->chunks = p.chunks;
+    a->max_splits = p.max_splits;
+    a->cluster = p.cluster;
+    a->max_clusters = p.max_clusters;
+}
+
+// The batched path (kv8_batch.cu): slots' q, k, v rows [slot][head][head_dim]
+// and positions from the QKV product, and rows to f16 pairs.
+struct SplitAttnArgs;
+cudaError_t launch_kv8_qkv_rows(uint32_t hd, const SplitAttnArgs& a, uint32_t slots, float* q, float* k, float* v,
+                                uint32_t* pos, uint32_t* row_start, cudaStream_t st);
+cudaError_t launch_kv8_to_pairs(const float* x, uint64_t n, uint16_t* hi, uint16_t* lo, cudaStream_t st);
+
 #ifdef __CUDACC__
 // Row `r` of the batch: its slot and position. False for a row that is not
 // there (behind the last sequence, no position, or past max_ctx: flagged).

@@ -37,7 +37,7 @@ struct hs_kv8_set {
     void** tab = nullptr;       // device: n region bases, n bitmaps, n tracking flags
     float* part = nullptr;      // records and counters of single-row attention (Kv8AttendArgs)
     uint32_t* counters = nullptr;
-    uint32_t max_splits = 0, cluster = 1, max_clusters = 0;
+    Kv8Plan plan;
     uint32_t* err = nullptr;    // device error word (ERR_POS)
     uint32_t* err_h = nullptr;  // pinned
     ~hs_kv8_set() {
@@ -191,18 +191,14 @@ int hs_kv8_set_new(hs_kv* const* kvs, uint32_t n, uint32_t n_heads, hs_kv8_set**
     HS_CUDA_TRY(cudaMemset(s->err, 0, 4));
     if (n_heads) {
         HS_CUDA_TRY(kv8_attend_set_smem_limits());
-        const uint32_t hd = s->spec.head_dim, nc = kv8_single_cols(n_heads / nkv);
-        const uint64_t items = (uint64_t)n * nkv * ((n_heads / nkv + nc - 1) / nc), least = kv8_min_split(hd);
-        s->max_splits = std::min<uint64_t>(kv8_max_splits(nkv), (s->spec.max_ctx + least - 1) / least);
-        while (s->cluster < 8 && s->cluster < s->max_splits) s->cluster *= 2;
-        s->max_clusters = (s->max_splits + s->cluster - 1) / s->cluster;
-        if (s->max_clusters > 1) {
-            if (cudaMalloc(&s->part, items * s->max_clusters * kv8_record(hd, nc) * 4) != cudaSuccess ||
-                cudaMalloc(&s->counters, items * 8 * 4) != cudaSuccess) {
+        s->plan = kv8_plan(s->spec, n_heads, n);
+        if (s->plan.counters) {
+            if (cudaMalloc(&s->part, s->plan.part_floats * 4) != cudaSuccess ||
+                cudaMalloc(&s->counters, s->plan.counters * 4) != cudaSuccess) {
                 cudaGetLastError();
                 return fail(HS_E_NOMEM, "8-bit set: out of memory");
             }
-            HS_CUDA_TRY(cudaMemset(s->counters, 0, items * 8 * 4));
+            HS_CUDA_TRY(cudaMemset(s->counters, 0, s->plan.counters * 4));
         }
     }
     HS_CUDA_TRY(cudaStreamSynchronize(nullptr));
@@ -278,16 +274,12 @@ int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t
     a.q = Kv8Mat{q, q_row_stride, q_head_stride, dtype};
     a.out = Kv8Mat{out, out_row_stride, out_head_stride, dtype};
     a.nh = s->nh;
-    a.group = s->nh / s->spec.n_kv_heads;
-    a.chunks = (a.group + kv8_single_cols(a.group) - 1) / kv8_single_cols(a.group);
+    kv8_use_plan(&a, s->plan);
     a.scale = scale;
     a.q_vec = fours(a.q);
     a.out_vec = fours(a.out);
     a.part = s->part;
     a.counters = s->counters;
-    a.max_splits = s->max_splits;
-    a.cluster = s->cluster;
-    a.max_clusters = s->max_clusters;
     return launched(launch_kv8_attend((uint32_t)hd, a, static_cast<cudaStream_t>(stream)), "attention");
 }
 
