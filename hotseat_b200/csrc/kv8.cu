@@ -1,8 +1,8 @@
 // The 8-bit KV cache: rows quantised as they are written, and read back.
 //
-// Both kernels move bytes once: a row of one head is taken by a team of
-// head_dim / 8 lanes, eight elements a lane (16 bytes of f16/bf16 or 32 of
-// f32 against 8 bytes of codes), so every access is a whole sector.
+// The kernels move bytes once: a row of one head is taken by head_dim / 8 lanes,
+// eight elements a lane (16 bytes of f16/bf16 or 32 of f32 against 8 bytes of
+// codes), so that accesses are whole sectors.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -79,24 +79,27 @@ __device__ __forceinline__ void store8(void* base, uint64_t e, const float* x) {
     }
 }
 
-// max|x|, with NaN kept: infinities and NaN both end as a scale of NaN.
-__device__ __forceinline__ float amax8(const float* x) {
-    float m = 0.0f;
-    bool bad = false;
+// max|x| as bits, whose order is that of the numbers, with infinities and then
+// NaN above them.
+__device__ __forceinline__ uint32_t amax8(const float* x) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        m = fmaxf(m, fabsf(x[i]));
-        bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-    }
-    return bad ? INFINITY : m;
+    for (int i = 0; i < 8; i++) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
 }
 
-// The scale that rows of largest magnitude m ask for: m times 1/127, both
+// The scale that rows of largest magnitude m (bits) ask for: m times 1/127, both
 // rounded to f32 (m / s is then at most 127 (1 + 2^-22), which rounds to 127).
-__device__ __forceinline__ float scale_for(float m) {
-    if (!(m <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
-    const float s = __fmul_rn(m, 1.0f / 127.0f);
+__device__ __forceinline__ float scale_for(uint32_t m) {
+    if (m >= 0x7f800000u) return __int_as_float(0x7fc00000);
+    const float s = __fmul_rn(__uint_as_float(m), 1.0f / 127.0f);
     return s < 1.17549435e-38f ? 0.0f : s;
+}
+// 1 / s to within 2^-23 of itself (s is normal, and so is 1 / s).
+__device__ __forceinline__ float reciprocal(float s) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
+    return y;
 }
 
 // The doublings k >= 0 that take the scale `held` to `need` or above (both
@@ -108,33 +111,40 @@ __device__ __forceinline__ int doublings(float held, float need) {
 }
 
 // Eight codes of x under scale s (not 0 or NaN): the integer nearest to x / s,
-// ties to even. x times the rounded reciprocal is off by at most 127 x 2^-23
-// of a step, so only a product that near to a half needs a second look: there
+// ties to even. x times the reciprocal is off by at most 127 x 2^-22 of a step,
+// so only a product that near to a half needs a second look: there
 // the remainder x - c s is exact in one FMA, and says which side x / s is on.
+// Adding 1.5 x 2^23 rounds to an integer, ties to even, and leaves it in the low
+// bits: no conversion instruction, a quarter as fast, is needed.
 __device__ __forceinline__ uint2 codes8(const float* x, float s, float inv) {
-    int c[8];
+    constexpr float kMagic = 12582912.0f;
+    uint32_t c[8];
     float near = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const float y = __fmul_rn(x[i], inv), r = rintf(y);
-        near = fmaxf(near, fabsf(__fsub_rn(y, r)));
-        c[i] = (int)r;
+        const float y = __fmul_rn(x[i], inv), m = __fadd_rn(y, kMagic);
+        near = fmaxf(near, fabsf(__fsub_rn(y, __fsub_rn(m, kMagic))));
+        c[i] = __float_as_uint(m);
     }
     if (near > 0.4999f) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float r2 = 2.0f * __fmaf_rn(-(float)c[i], s, x[i]);
+            const float r2 = 2.0f * __fmaf_rn(-__fsub_rn(__uint_as_float(c[i]), kMagic), s, x[i]);
             if (r2 > s || (r2 == s && (c[i] & 1))) c[i]++;
             else if (r2 < -s || (r2 == -s && (c[i] & 1))) c[i]--;
         }
     }
-    uint32_t w[2] = {0, 0};
+    return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
+}
+
+// The values of eight codes under scale s: a byte with its sign bit flipped,
+// under the exponent of 2^23, is 2^23 + 128 + code, exactly.
+__device__ __forceinline__ void values8(uint2 c, float s, float* x) {
+    const uint32_t w[2] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u};
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        c[i] = max(-127, min(127, c[i]));
-        w[i >> 2] |= (uint32_t)(c[i] & 0xff) << (8 * (i & 3));
-    }
-    return make_uint2(w[0], w[1]);
+    for (int e = 0; e < 8; e++)
+        x[e] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w[e >> 2], 0x4b000000u, 0x7440 | (e & 3))), 8388736.0f), s);
 }
 
 // Sets the page bits of `len` bytes at `off`, after they are visible (a
@@ -148,38 +158,125 @@ __device__ __forceinline__ bool tracked(const Kv8View& kv, uint32_t slot) {
     return *reinterpret_cast<const volatile uint32_t*>(kv.tracking[slot]) != 0;
 }
 
-// Append, a scale for every position: a team per (row, head, K or V).
+// What one lane takes of a row: piece c of the row's 2 x nkv x HD / 8 pieces of
+// eight elements, K's heads first.
+template <int HD>
+struct Piece {
+    uint32_t v, head, e;  // 1 for V, the head, the first element
+    __device__ __forceinline__ Piece(uint32_t c, uint32_t nkv) {
+        const uint32_t h = c / (HD / 8);
+        v = h >= nkv ? 1 : 0;
+        head = h - v * nkv;
+        e = c % (HD / 8) * 8;
+    }
+};
+
+// How many of n ascending values f(0), f(1), ... are at most `limit`: the lanes
+// of a (converged) warp look at 32 at once, one trip to memory for up to 128,
+// where a search by halves takes one a step.
+template <typename F>
+__device__ __forceinline__ uint32_t count_upto(uint32_t n, uint64_t limit, F f) {
+    const uint32_t lane = threadIdx.x & 31;
+    if (n > 512) {
+        uint32_t lo = 0, hi = n;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (f(mid) <= limit) lo = mid + 1;
+            else hi = mid;
+        }
+        return lo;
+    }
+    uint32_t count = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < n; i += 32) count += __popc(__ballot_sync(0xffffffffu, i + lane < n && f(i + lane) <= limit));
+    return count;
+}
+
+// The rows that one warp walks: where row r lies, and how many from it on lie
+// behind one another in the same slot.
+struct Walk {
+    uint8_t* base = nullptr;
+    uint32_t slot = 0, first = 0, end = 0, p0 = 0;
+    // False: no place for row r (behind the last sequence, no position, past max_ctx).
+    __device__ __forceinline__ bool to(const Kv8View& kv, const Kv8Rows& rows, uint32_t r, uint32_t last, uint32_t* pos,
+                                       uint32_t* n) {
+        if (r < first || r >= end) {
+            if (rows.row_start) {
+                slot = count_upto(rows.n_slots, r, [&](uint32_t i) { return __ldg(rows.row_start + i + 1); });
+                first = slot < rows.n_slots ? __ldg(rows.row_start + slot) : r;
+                end = slot < rows.n_slots ? __ldg(rows.row_start + slot + 1) : last;
+                if (first > r) first = r, end = r + 1, slot = rows.n_slots;
+            } else {
+                slot = first = r;
+                end = r + 1;
+            }
+            p0 = slot < rows.n_slots ? __ldg(rows.pos + slot) : kPosNone;
+            base = slot < rows.n_slots ? reinterpret_cast<uint8_t*>(kv.base[slot]) : nullptr;
+        }
+        *n = min(end, last) - r;
+        if (p0 == kPosNone) return false;
+        const uint64_t p = (uint64_t)p0 + (r - first);
+        if (p >= kv.max_ctx) {
+            atomicOr(rows.err, ERR_POS);
+            return false;
+        }
+        *n = (uint32_t)min((uint64_t)*n, kv.max_ctx - p);
+        *pos = (uint32_t)p;
+        return true;
+    }
+};
+
+// Append, a scale for every position: a warp takes `per` rows in turn, HD / 8
+// lanes a head. The row's slot is searched once a row, the same for all lanes.
 template <int HD, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
-                                                          const Kv8Mat v) {
-    constexpr uint32_t TL = HD / 8, TEAMS = kThreads / TL;
-    const uint32_t tl = threadIdx.x % TL;
-    const uint64_t item = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / TL;
-    const uint64_t r64 = item / (2 * kv.nkv);
-    const uint32_t which = (uint32_t)(item - r64 * 2 * kv.nkv), is_v = which >= kv.nkv ? 1 : 0;
-    const uint32_t head = which - is_v * kv.nkv;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    uint32_t slot = 0, pos = 0;
-    const bool live = r64 < rows.n_rows && kv8_place(rows, kv.max_ctx, (uint32_t)r64, &slot, &pos);
-    const Kv8Mat& m = is_v ? v : k;
-    if (live) load8<DT, VEC>(m.p, r64 * m.row + head * m.head + 8 * tl, x);
-    float top = amax8(x);
+                                                          const Kv8Mat v, uint32_t per) {
+    constexpr uint32_t TL = HD / 8;
+    const uint32_t lane = threadIdx.x & 31, pieces = 2 * kv.nkv * TL;
+    const uint32_t first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * per, last = min(first + per, rows.n_rows);
+    constexpr uint32_t N = 4;
+    Walk walk;
+    uint32_t n, pos;
+    for (uint32_t r0 = first; r0 < last; r0 += n) {
+        if (!walk.to(kv, rows, r0, last, &pos, &n)) continue;
+        n = min(n, N);
+        for (uint32_t c0 = 0; c0 < pieces; c0 += 32) {
+            const uint32_t c = c0 + lane;
+            const bool in = c < pieces;
+            const Piece<HD> p(in ? c : 0, kv.nkv);
+            const Kv8Mat& m = p.v ? v : k;
+            float x[N][8];
+            uint32_t top[N];
 #pragma unroll
-    for (uint32_t o = TL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!live) return;
-    const float s = scale_for(top);
-    uint2 c = make_uint2(0, 0);
-    if (s > 0.0f) c = codes8(x, s, __fdiv_rn(1.0f, s));
-    uint8_t* base = reinterpret_cast<uint8_t*>(kv.base[slot]);
-    const uint64_t at = kv.code_off(is_v, head, pos), sat = kv.scale_off(is_v, head, pos);
-    *reinterpret_cast<uint2*>(base + at + 8 * tl) = c;
-    if (tl == 0) *reinterpret_cast<float*>(base + sat) = s;
-    if (tracked(kv, slot)) {
-        __threadfence();
-        __syncwarp(__activemask());
-        if (tl == 0) {
-            mark_pages(kv, slot, at, HD);
-            mark_pages(kv, slot, sat, 4);
+            for (uint32_t i = 0; i < N; i++) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
+                if (in && i < n) load8<DT, VEC>(m.p, (r0 + i) * m.row + p.head * m.head + p.e, x[i]);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) {
+                top[i] = amax8(x[i]);
+#pragma unroll
+                for (uint32_t o = TL / 2; o > 0; o >>= 1) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+            }
+            uint8_t* code = walk.base + kv.code_off(p.v, p.head, pos) + p.e;
+            uint8_t* scale = walk.base + kv.scale_off(p.v, p.head, pos);
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++, code += kv.pos_stride, scale += 4 * kv.sblk_stride)
+                if (in && i < n) {
+                    const float s = scale_for(top[i]);
+                    *reinterpret_cast<uint2*>(code) = s > 0.0f ? codes8(x[i], s, reciprocal(s)) : make_uint2(0, 0);
+                    if (p.e == 0) *reinterpret_cast<float*>(scale) = s;
+                }
+        }
+        if (tracked(kv, walk.slot)) {
+            __threadfence();
+            __syncwarp();
+            for (uint32_t h = lane; h < 2 * kv.nkv * n; h += 32) {
+                const uint32_t i = h / (2 * kv.nkv), w = h / kv.nkv & 1, head = h % kv.nkv;
+                mark_pages(kv, walk.slot, kv.code_off(w, head, pos + i), HD);
+                mark_pages(kv, walk.slot, kv.scale_off(w, head, pos + i), 4);
+            }
         }
     }
 }
@@ -194,40 +291,33 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
                                                             const Kv8Mat v) {
     constexpr uint32_t TL = HD / 8, RPW = 32 / TL;
     constexpr uint32_t WPU = B / (4 * RPW) > 8 ? 8 : B / (4 * RPW), RL = B / (WPU * RPW), UPC = 8 / WPU;
-    __shared__ float tops[8];
+    __shared__ uint32_t tops[8];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tl = lane % TL;
     const uint32_t j0 = (warp % WPU) * RPW + lane / TL;  // this lane's rows of the block: j0 + i * WPU * RPW
-    const uint64_t unit = (uint64_t)blockIdx.x * UPC + warp / WPU;
-    const uint64_t u64 = unit / (2 * kv.nkv);
-    const uint32_t which = (uint32_t)(unit - u64 * 2 * kv.nkv), is_v = which >= kv.nkv ? 1 : 0;
+    const uint32_t unit = blockIdx.x * UPC + warp / WPU, blk_no = unit / (2 * kv.nkv);  // the check on rows keeps units in 32 bits
+    const uint32_t which = unit - blk_no * 2 * kv.nkv, is_v = which >= kv.nkv ? 1 : 0;
     const uint32_t head = which - is_v * kv.nkv;
 
     // the unit's slot, its rows [r0, r0 + m) and its block
     uint32_t slot = 0, r0 = 0, m = 0, p0 = kPosNone, blk = 0;
     bool live;
     if (!rows.row_start) {
-        slot = r0 = (uint32_t)u64;
-        live = u64 < rows.n_rows;
+        slot = r0 = (uint32_t)blk_no;
+        live = blk_no < rows.n_rows;
         m = 1;
         if (live) p0 = __ldg(rows.pos + slot);
         blk = p0 / B;
     } else {
-        uint32_t lo = 0, hi = rows.n_slots;  // the last slot whose first unit is <= u64
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (__ldg(rows.row_start + mid) / B + 2ull * mid <= u64)
-                lo = mid + 1;
-            else
-                hi = mid;
-        }
-        live = lo > 0;
+        // the last slot whose first unit is <= blk_no
+        const uint32_t upto = count_upto(rows.n_slots, blk_no, [&](uint32_t i) { return __ldg(rows.row_start + i) / B + 2ull * i; });
+        live = upto > 0;
         if (live) {
-            slot = lo - 1;
+            slot = upto - 1;
             r0 = __ldg(rows.row_start + slot);
             const uint32_t end = min(__ldg(rows.row_start + slot + 1), rows.n_rows);
             m = end > r0 ? end - r0 : 0;
             p0 = __ldg(rows.pos + slot);
-            blk = p0 / B + (uint32_t)(u64 - (r0 / B + 2ull * slot));
+            blk = p0 / B + (uint32_t)(blk_no - (r0 / B + 2ull * slot));
         }
     }
     live = live && m > 0 && p0 != kPosNone;
@@ -237,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
     live = live && b0 < kv.max_ctx;
 
     float x[RL][8];
-    float top = 0.0f;
+    uint32_t top = 0;
     const Kv8Mat& mat = is_v ? v : k;
 #pragma unroll
     for (uint32_t i = 0; i < RL; i++) {
@@ -246,15 +336,15 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
         for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
         if (live && p >= p0 && p < end && p < kv.max_ctx)
             load8<DT, VEC>(mat.p, (r0 + (p - p0)) * mat.row + head * mat.head + 8 * tl, x[i]);
-        top = fmaxf(top, amax8(x[i]));
+        top = max(top, amax8(x[i]));
     }
 #pragma unroll
-    for (uint32_t o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (uint32_t o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (WPU > 1) {
         if (lane == 0) tops[warp] = top;
         __syncthreads();
 #pragma unroll
-        for (uint32_t w = 0; w < WPU; w++) top = fmaxf(top, tops[warp / WPU * WPU + w]);
+        for (uint32_t w = 0; w < WPU; w++) top = max(top, tops[warp / WPU * WPU + w]);
     }
     uint8_t* base = live ? reinterpret_cast<uint8_t*>(kv.base[slot]) : nullptr;
     const uint64_t sat = kv.scale_off(is_v, head, blk);
@@ -269,7 +359,7 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
         if (s > 0.0f) k2 = doublings(held, s);
         s = __fmul_rn(__fmul_rn(held, pow2i(k2 / 2)), pow2i(k2 - k2 / 2));  // 2^k2 itself may pass f32
     }
-    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    const float inv = s > 0.0f ? reciprocal(s) : 0.0f;
     const bool track = tracked(kv, slot);
 #pragma unroll
     for (uint32_t i = 0; i < RL; i++) {
@@ -306,28 +396,44 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
     }
 }
 
-// Read back: a team per (row, head, K or V).
+// Read back: as k_append_rows, four rows' pieces in flight at once.
 template <int HD, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_read_rows(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
-                                                        const Kv8Mat v) {
-    constexpr uint32_t TL = HD / 8, TEAMS = kThreads / TL;
-    const uint32_t tl = threadIdx.x % TL;
-    const uint64_t item = (uint64_t)blockIdx.x * TEAMS + threadIdx.x / TL;
-    const uint64_t r64 = item / (2 * kv.nkv);
-    const uint32_t which = (uint32_t)(item - r64 * 2 * kv.nkv), is_v = which >= kv.nkv ? 1 : 0;
-    const uint32_t head = which - is_v * kv.nkv;
-    uint32_t slot = 0, pos = 0;
-    if (r64 >= rows.n_rows || !kv8_place(rows, kv.max_ctx, (uint32_t)r64, &slot, &pos)) return;
-    const Kv8Mat& m = is_v ? v : k;
-    if (!m.p) return;
-    const uint8_t* base = reinterpret_cast<const uint8_t*>(kv.base[slot]);
-    const uint2 c = *reinterpret_cast<const uint2*>(base + kv.code_off(is_v, head, pos) + 8 * tl);
-    const float s = *reinterpret_cast<const float*>(base + kv.scale_off(is_v, head, pos >> kv.block_shift));
-    float x[8];
+                                                        const Kv8Mat v, uint32_t per) {
+    constexpr uint32_t TL = HD / 8, AT_ONCE = 4;
+    const uint32_t lane = threadIdx.x & 31, pieces = 2 * kv.nkv * TL;
+    const uint32_t first = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * per, last = min(first + per, rows.n_rows);
+    Walk walk;
+    uint32_t n, pos;
+    for (uint32_t r0 = first; r0 < last; r0 += n) {
+        if (!walk.to(kv, rows, r0, last, &pos, &n)) continue;
+        n = min(n, AT_ONCE);
+        for (uint32_t c = lane; c < pieces; c += 32) {
+            const Piece<HD> p(c, kv.nkv);
+            const Kv8Mat& m = p.v ? v : k;
+            if (!m.p) continue;
+            uint2 code[AT_ONCE];
+            float s[AT_ONCE];
+            const uint8_t* from = walk.base + kv.code_off(p.v, p.head, pos) + p.e;
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = __fmul_rn((float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))), s);
-    store8<DT, VEC>(const_cast<void*>(m.p), r64 * m.row + head * m.head + 8 * tl, x);
+            for (uint32_t i = 0; i < AT_ONCE; i++, from += kv.pos_stride)
+                if (i < n) {
+                    code[i] = __ldg(reinterpret_cast<const uint2*>(from));
+                    s[i] = __ldg(reinterpret_cast<const float*>(walk.base + kv.scale_off(p.v, p.head, (pos + i) >> kv.block_shift)));
+                }
+#pragma unroll
+            for (uint32_t i = 0; i < AT_ONCE; i++)
+                if (i < n) {
+                    float x[8];
+                    values8(code[i], s[i], x);
+                    store8<DT, VEC>(const_cast<void*>(m.p), (r0 + i) * m.row + p.head * m.head + p.e, x);
+                }
+        }
+    }
 }
+
+// Rows a warp takes: one while that leaves SMs idle, eight from 16 warps an SM on.
+uint32_t rows_per_warp(uint32_t n_rows) { return n_rows >= 148 * 16 * 8 ? 8 : n_rows >= 148 * 16 * 4 ? 4 : 1; }
 
 bool vec_ok(const Kv8Mat& m) {
     const uint64_t b = dtype_bytes(m.dtype);
@@ -352,8 +458,8 @@ void append_hd(const Kv8View& kv, const Kv8Rows& rows, const Kv8Mat& k, const Kv
         constexpr int DT = decltype(dt)::value;
         constexpr bool VEC = decltype(vec)::value;
         if (kv.block_shift == 0) {
-            const uint64_t items = (uint64_t)rows.n_rows * 2 * kv.nkv, per = kThreads / (HD / 8);
-            k_append_rows<HD, DT, VEC><<<(uint32_t)((items + per - 1) / per), kThreads, 0, st>>>(kv, rows, k, v);
+            const uint32_t per = rows_per_warp(rows.n_rows), cta = per * (kThreads / 32);
+            k_append_rows<HD, DT, VEC><<<(rows.n_rows + cta - 1) / cta, kThreads, 0, st>>>(kv, rows, k, v, per);
             return;
         }
         const uint32_t B = 1u << kv.block_shift;
@@ -388,10 +494,9 @@ cudaError_t launch_kv8_read(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows,
     by_type(k.dtype, vec, [&](auto dt, auto ve) {
         constexpr int DT = decltype(dt)::value;
         constexpr bool VEC = decltype(ve)::value;
-        const uint64_t items = (uint64_t)rows.n_rows * 2 * kv.nkv, per = kThreads / (hd / 8);
-        const uint32_t grid = (uint32_t)((items + per - 1) / per);
-        if (hd == 64) k_read_rows<64, DT, VEC><<<grid, kThreads, 0, st>>>(kv, rows, k, v);
-        else k_read_rows<128, DT, VEC><<<grid, kThreads, 0, st>>>(kv, rows, k, v);
+        const uint32_t per = rows_per_warp(rows.n_rows), cta = per * (kThreads / 32), grid = (rows.n_rows + cta - 1) / cta;
+        if (hd == 64) k_read_rows<64, DT, VEC><<<grid, kThreads, 0, st>>>(kv, rows, k, v, per);
+        else k_read_rows<128, DT, VEC><<<grid, kThreads, 0, st>>>(kv, rows, k, v, per);
     });
     return cudaGetLastError();
 }

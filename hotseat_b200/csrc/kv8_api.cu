@@ -60,8 +60,8 @@ int check_call(const hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint3
     if (dtype > HS_BF16) return fail(HS_E_ARG, "unknown element type");
     if (!pos) return fail(HS_E_ARG, "null positions");
     if (!row_start && n_rows != s->n) return fail(HS_E_ARG, "without row_start there is one row for each slot");
-    // grid sizes: items of 2 x KV heads (or query heads) a row in 31 bits
-    if ((uint64_t)n_rows * 2 * std::max(s->spec.n_kv_heads, s->nh) > 0x7fffffffull)
+    // grids and the blocks' numbers (n_rows + 2 n_slots at most, for each head of K and V) in 31 bits
+    if (((uint64_t)n_rows + 2ull * s->n) * 2 * std::max(s->spec.n_kv_heads, s->nh) > 0x7fffffffull)
         return fail(HS_E_UNSUPPORTED, "too many rows in one call");
     return HS_OK;
 }
