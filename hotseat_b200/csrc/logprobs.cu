@@ -91,14 +91,31 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
         if (isnan(x.l) || isnan(x.t)) {
             r.l = r.t = __longlong_as_double(0x7ff8000000000000ll);
         } else if (x.l != 0.0) {
-            const double d = (double)x.m - (double)r.m, w = exp(d);
+            // d <= 0 and the weight in f32: off by 2^-22 at d = 0 (where it is 1), less
+            // of the whole the further below
+            const float d = fmaxf(__fsub_rn(x.m, r.m), -200.0f);
+            const double w = d == 0.0f ? 1.0 : (double)ex2(__fmul_rn(d, kLog2e));
             r.l += x.l * w;
-            r.t += (x.t + x.l * d) * w;
+            r.t += (x.t + x.l * (double)d) * w;
         }
     };
     add(a);
     add(b);
     return r;
+}
+
+// Lanes 0 .. n - 1's (n a power of two) as one, pairs first: in lane 0.
+__device__ __forceinline__ Sums join_lanes(Sums x, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t o = 1; o < n; o <<= 1) {
+        Sums y;
+        y.l = __shfl_xor_sync(0xffffffffu, x.l, o);
+        y.t = __shfl_xor_sync(0xffffffffu, x.t, o);
+        y.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+        y.before = __shfl_xor_sync(0xffffffffu, x.before, o);
+        x = lane & o ? join(y, x) : join(x, y);
+    }
+    return x;
 }
 
 struct Shared {
@@ -110,9 +127,8 @@ struct Shared {
     uint64_t best[kThreads];       // ... of a thread (the second way)
     uint64_t cand[kCand];
     uint64_t all[kCluster * kLogprobTop];
-    // what the other CTAs of the row read: the top tokens in order (0: none), the sums
-    uint64_t top[kLogprobTop];
-    Sums sums;
+    uint64_t top[kLogprobTop];     // the top tokens so far, in order (0: none)
+    Sums sums[kCluster];           // the first CTA's: every CTA's sums, and top tokens in `all`
 };
 
 // Logit i = (j * 512 + tid) * V + e of a strip is this thread's number V j + e.
@@ -135,6 +151,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
     const uint32_t id = a.ids ? __ldg(a.ids + r) : 0xffffffffu;
     const float xt = id < a.vocab ? logit<DT>(row, id) : __int_as_float(0x7fc00000);
     const uint32_t begin = min(rank * share, a.vocab), end = min(begin + share, a.vocab);
+    // every CTA of the cluster is there before one writes to the first
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     Sums sums;
     if (tid < kLogprobTop) s.top[tid] = 0;
 
@@ -165,18 +183,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 for (uint32_t e = 0; e < V; e++) x[V * j + e] = i + e < n ? logit<DT>(mine, i + e) : -INFINITY;
             }
         }
-        // the strip's maximum (NaN skipped: it shows in the sums)
+        // the warp's maximum (NaN skipped: it shows in the sums), under which its sums stand
         float m = -INFINITY;
 #pragma unroll
         for (uint32_t k = 0; k < kPer; k++) m = fmaxf(m, x[k]);
         const float mine_top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) s.m[warp] = m;
         if (tid == 0) s.n_cand = 0, s.bound = 0;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < 16; w++) m = fmaxf(m, s.m[w]);
 
         // Sums over eight logits in f32, over more in f64. A logit 200 below the
         // maximum has no weight, and its distance is cut there: 0 times -inf is not.
@@ -201,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
             unpack2(ts, &t0, &t1);
             l += (double)(l0 + l1), t += (double)(t0 + t1);
         }
+        const bool nan = isnan(l);  // one of the thread's logits is, or +inf among them
         uint32_t before = 0;
         if (a.rank && id < a.vocab) {
             if (isnan(xt)) {  // before it: NaNs of lower ids
@@ -211,10 +226,25 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 // bound of xt or of the number just under it (none under -inf: NaN)
                 float under = xt == 0.0f ? __int_as_float(0x80000001u) : __int_as_float(__float_as_int(xt) + (xt < 0.0f ? 1 : -1));
                 if (xt == -INFINITY) under = __int_as_float(0x7fc00000);
+                // V logits at once lie on one side of the id, but for the V that hold it
 #pragma unroll
-                for (uint32_t k = 0; k < kPer; k++) {
-                    const uint32_t p = place<V>(k);
-                    before += p < n && !(x[k] <= (from + p < id ? under : xt)) ? 1 : 0;
+                for (uint32_t j = 0; j < kPer / V; j++) {
+                    const uint32_t p = place<V>(V * j), first = from + p;
+                    const float limit = first + V <= id ? under : xt;
+#pragma unroll
+                    for (uint32_t e = 0; e < V; e++) before += !(x[V * j + e] <= limit) ? 1 : 0;
+                    if (first < id && id < first + V) {
+#pragma unroll
+                        for (uint32_t e = 0; e < V; e++) before += x[V * j + e] == xt && first + e < id ? 1 : 0;
+                    }
+                }
+                // the strip's filling, -inf, is before nothing; but `under` is NaN for a token of -inf
+                if (xt == -INFINITY) {
+#pragma unroll
+                    for (uint32_t j = 0; j < kPer / V; j++)
+#pragma unroll
+                        for (uint32_t e = 0; e < V; e++)
+                            if (place<V>(V * j + e) >= n && from + place<V>(V * j) + V <= id) before--;
                 }
             }
         }
@@ -224,17 +254,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
             t += __shfl_xor_sync(0xffffffffu, t, o);
             before += __shfl_xor_sync(0xffffffffu, before, o);
         }
-        if (lane == 0) s.l[warp] = l, s.t[warp] = t, s.before[warp] = before;
+        if (lane == 0) s.l[warp] = l, s.t[warp] = t, s.m[warp] = m, s.before[warp] = before;
 
         if (a.top) {
             // the thread's largest key: a NaN, else its largest logit, the first of equal ones
-            uint32_t at = kPer;
-            bool nan = false;
+            uint32_t at = 0;
 #pragma unroll
             for (uint32_t i = 0; i < kPer; i++) {
                 const uint32_t k = kPer - 1 - i;
-                if (!(x[k] < mine_top)) at = k;
-                nan |= isnan(x[k]);
+                if (x[k] == mine_top) at = k;
             }
             uint64_t best = 0;
             if (nan || mine_top == -INFINITY) {
@@ -308,32 +336,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
             }
         }
         __syncthreads();
-        Sums strip;
-        strip.m = m;
-#pragma unroll
-        for (int w = 0; w < 16; w++) strip.l += s.l[w], strip.t += s.t[w], strip.before += s.before[w];
-        if (m == -INFINITY && !isnan(strip.l)) strip.l = strip.t = 0.0;
-        sums = from == begin ? strip : join(sums, strip);
+        // the warps' sums as the CTA's, by the first warp: lanes 0 .. 15, pairs first
+        if (warp == 0) {
+            Sums strip;
+            if (lane < 16) {
+                strip.l = s.l[lane], strip.t = s.t[lane], strip.m = s.m[lane], strip.before = s.before[lane];
+                if (strip.m == -INFINITY && !isnan(strip.l)) strip.l = strip.t = 0.0;
+            }
+            strip = join_lanes(strip, 16);
+            sums = from == begin ? strip : join(sums, strip);
+        }
         __syncthreads();  // the arrays are free for the next strip
     }
-    if (tid == 0) s.sums = sums;
-    cl.sync();
+    // results go to the cluster's first CTA; the others are done then
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    Shared& to = *cl.map_shared_rank(&s, 0);
     const uint32_t nk = ctas * a.top;
-    if (rank == 0) {  // the CTAs' results, then they may leave
-        if (tid < ctas) sums = *cl.map_shared_rank(&s.sums, tid);
-        for (uint32_t i = tid; i < nk; i += kThreads) s.all[i] = cl.map_shared_rank(s.top, i / a.top)[i % a.top];
-    }
-    cl.sync();
+    if (tid == 0) to.sums[rank] = sums;
+    if (tid < a.top) to.all[rank * a.top + tid] = s.top[tid];
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (rank != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp == 0) {
-        for (uint32_t o = 1; o < ctas; o <<= 1) {  // lanes 0 .. ctas - 1, a power of two
-            Sums other;
-            other.l = __shfl_xor_sync(0xffffffffu, sums.l, o);
-            other.t = __shfl_xor_sync(0xffffffffu, sums.t, o);
-            other.m = __shfl_xor_sync(0xffffffffu, sums.m, o);
-            other.before = __shfl_xor_sync(0xffffffffu, sums.before, o);
-            sums = lane & o ? join(other, sums) : join(sums, other);
-        }
+        if (lane < ctas) sums = s.sums[lane];
+        sums = join_lanes(sums, ctas);
         // nothing but -inf, or +inf: no distribution
         if (sums.m == -INFINITY || sums.m == INFINITY) sums.l = sums.t = __longlong_as_double(0x7ff8000000000000ll);
         const double lz = log(sums.l);
