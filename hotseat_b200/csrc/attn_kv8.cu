@@ -7,11 +7,14 @@
 // 16-bit rows, after scaling by powers of two that keep it in f16's range:
 //   q:       its largest element to [2^13, 2^14)
 //   weights: w = exp(S - m) s_v 2^(10 - e), 2^e at or above the largest s_v so
-//            far, so that weights down to 2^-34 of the largest still count
+//            far (of all that the CTA will meet, in chunks), so that weights down
+//            to 2^-34 of the largest still count
 // Scores, statistics and sums are f32.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 #include "common.h"
 #include "device.cuh"
@@ -154,6 +157,13 @@ __device__ __forceinline__ void cp_async_wait() {
 // The splits are joined in two levels: those of a cluster (up to 8) through
 // distributed shared memory, each CTA a share of the outputs; where a row has
 // more, each share's last cluster joins the clusters' records in order.
+//
+// Bound by the instructions between a block's arrival and the next (about 515
+// a warp for 4 KB of codes, in a chain of ~1,700 clocks; four warps an SM
+// quarter hide part of it) and, below ~2,000 positions, by the CTA's start and
+// join. 64 rows of 14/2 heads of 64, f32, up to 2,048 positions: 15 us, 3.6 at
+// the memory's rate; 8,192 positions each: 46 us (2.9 TB/s of codes); one row:
+// 5.9 us at 2,048 positions, 16 at 32,768 (12/2 heads of 128).
 template <int HD, int DT, int NT>
 struct DecGeom {
     static constexpr uint32_t BP = HD == 64 ? 32 : 16;  // positions of a block: 4 KB of codes either way
@@ -565,6 +575,18 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 //   O' = W V     A = W (TMEM),   B = V^T (shared), 128 x head_dim
 //
 // While one row tile's threads are at their softmax the other's products run.
+//
+// SPLIT: few rows over many positions (kv8_chunk_shared), which would leave
+// most SMs idle. A cluster's CTAs take the positions in equal runs of steps,
+// leave outputs, maxima and sums in shared memory, and each joins a share of
+// the rows.
+//
+// Bound by the row warps' softmax (exponentials, pairs, TMEM round trips; about
+// 3,100 clocks for 128 x 128 scores a warp in bf16, 5,800 with f32's pairs)
+// and by the CTA's start (12,000 clocks: q, the scales' maxima, the first
+// codes), not by the products. 12/2 heads of 128, 2,048 rows a slot: 8 slots in
+// bf16 205 us (502 TFLOP/s of the 1,630 measured); 4 in f32 183 us (282, each
+// product of pairs counted once).
 template <int HD, int DT>
 struct ChunkGeom {
     static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
@@ -582,6 +604,7 @@ struct ChunkGeom {
     static constexpr uint32_t Q_AT = 0, K_AT = Q_AT + 2 * (QPAIR ? 2 : 1) * Q_BYTES, V_AT = K_AT + NB * K_BYTES;
     static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: K [NB][128], V [NB][128]
     static constexpr uint32_t BYTES = SC_AT + (DT == HS_BF16 ? 0 : NB * 2 * KT * 4) + 1024;
+    static_assert(SC_AT >= ROWS * HD * 4, "the outputs fit where the operands were");
     static constexpr uint32_t S_COL = 0, O_COL = 256;       // TMEM columns: S of both tiles, O' of both
     // bf16 rows take the scales with the codes (K and V rounded to f16, 2^-11 a
     // value against the 2^-8 of their own type): 2.5 operations a score less.
@@ -627,7 +650,11 @@ __device__ __forceinline__ void bar_sync(uint32_t id) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
-template <int HD, int DT>
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int HD, int DT, bool SPLIT>
 __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(const Kv8AttendArgs a) {
     using G = ChunkGeom<HD, DT>;
     constexpr uint32_t KT = G::KT, NB = G::NB;
@@ -637,27 +664,41 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
     __shared__ uint32_t tmem_slot;
     __shared__ float ktop[16], vtop[16], row_cf[G::ROWS];
     __shared__ uint64_t row_q[G::ROWS], row_out[G::ROWS];  // element offsets of the tile's rows
+    __shared__ float row_m[SPLIT ? G::ROWS : 1], row_l[SPLIT ? G::ROWS : 1];
     // the warp's number as a value that is the same for its lanes
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t group = a.group;
 
     // the tile: slot, its rows' first pair, its last position. Tiles of slot i
     // start at row_start[i] * group / 256 + i, room for all that it can have.
-    const uint32_t bt = gridDim.x / a.kv.nkv - 1 - blockIdx.x / a.kv.nkv, kvh = blockIdx.x % a.kv.nkv;  // long ones first
-    uint32_t lo = 0, hi = a.rows.n_slots;
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if ((uint64_t)__ldg(a.rows.row_start + mid) * group / G::ROWS + mid <= bt)
-            lo = mid + 1;
-        else
-            hi = mid;
+    const uint32_t part = SPLIT ? blockIdx.x % kKv8ChunkSplits : 0, at = SPLIT ? blockIdx.x / kKv8ChunkSplits : blockIdx.x;
+    const uint32_t n_at = SPLIT ? gridDim.x / kKv8ChunkSplits : gridDim.x;
+    const uint32_t bt = n_at / a.kv.nkv - 1 - at / a.kv.nkv;  // long ones first
+    uint32_t slot, kvh = at % a.kv.nkv;
+    uint64_t f0 = 0;
+    if (SPLIT && a.slot_clusters) {
+        slot = at / a.slot_clusters;
+        kvh = at % a.slot_clusters % a.kv.nkv;
+        f0 = (uint64_t)(at % a.slot_clusters / a.kv.nkv) * G::ROWS;
+    } else {
+        uint32_t lo = 0, hi = a.rows.n_slots;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if ((uint64_t)__ldg(a.rows.row_start + mid) * group / G::ROWS + mid <= bt)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        if (lo == 0) return;
+        slot = lo - 1;
+        f0 = (bt - ((uint64_t)__ldg(a.rows.row_start + slot) * group / G::ROWS + slot)) * G::ROWS;
     }
-    if (lo == 0) return;
-    const uint32_t slot = lo - 1, r0 = __ldg(a.rows.row_start + slot);
+    const uint32_t r0 = __ldg(a.rows.row_start + slot);
     const uint32_t r1 = min(__ldg(a.rows.row_start + slot + 1), a.rows.n_rows), m = r1 > r0 ? r1 - r0 : 0;
-    const uint64_t f0 = (bt - ((uint64_t)r0 * group / G::ROWS + slot)) * G::ROWS, pairs = (uint64_t)m * group;
-    if (f0 >= pairs) return;
+    const uint64_t pairs = (uint64_t)m * group;
     const uint32_t pos0 = __ldg(a.rows.pos + slot);
+    if (SPLIT != (pos0 < a.kv.max_ctx && kv8_chunk_shared((pairs + G::ROWS - 1) / G::ROWS, pos0, a.kv.nkv))) return;
+    if (f0 >= pairs) return;
     const uint32_t live = (uint32_t)min((uint64_t)G::ROWS, pairs - f0);  // pairs of this CTA
     const uint32_t jlast = (uint32_t)((f0 + live - 1) / group);          // its last row
     if (pos0 == kPosNone || (uint64_t)pos0 + (uint32_t)(f0 / group) >= a.kv.max_ctx) {  // nothing to see
@@ -670,7 +711,10 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
     }
     const uint64_t plast = (uint64_t)pos0 + jlast;
     if (plast >= a.kv.max_ctx && tid == 0) atomicOr(a.rows.err, ERR_POS);
-    const uint32_t end = (uint32_t)min(plast + 1, (uint64_t)a.kv.max_ctx);  // positions seen: [0, end)
+    const uint32_t seen = (uint32_t)min(plast + 1, (uint64_t)a.kv.max_ctx);  // positions [0, seen)
+    // this CTA's positions: [first, first + end), whole tiles but for the last
+    const uint32_t all = (seen + KT - 1) / KT, first = SPLIT ? all * part / kKv8ChunkSplits * KT : 0;
+    const uint32_t end = (SPLIT ? min(seen, all * (part + 1) / kKv8ChunkSplits * KT) : seen) - first;
     const uint32_t tiles = (end + KT - 1) / KT;
     const uint32_t users = live > 128 ? 2 : 1;  // row tiles at work
 
@@ -693,8 +737,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
     }
     // the largest scales that this CTA will meet, and powers of two to put them under
     const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
-    const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, 0));
-    const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, 0));
+    const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, first >> a.kv.block_shift));
+    const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, first >> a.kv.block_shift));
     {
         float kt = 0.0f, vt = 0.0f;
         for (uint32_t i = tid; i <= (end - 1) >> a.kv.block_shift; i += G::THREADS) {
@@ -752,8 +796,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         // pieces fall into different banks; the outputs' columns follow.
         constexpr uint32_t DW = HD / 4, VP = HD / 64;
         const uint32_t dw = lane % DW, vg = 2 * cw + lane / DW;
-        const uint8_t* kp = base + a.kv.code_off(0, kvh, 0) + 16 * kc;
-        const uint8_t* vp = base + a.kv.code_off(1, kvh, 0) + 4 * dw;
+        const uint8_t* kp = base + a.kv.code_off(0, kvh, first) + 16 * kc;
+        const uint8_t* vp = base + a.kv.code_off(1, kvh, first) + 4 * dw;
         uint4 kw[G::SUB][KP];
         uint32_t vw[G::SUB][VP][8];
         float ks[G::SUB], vs[G::SUB];
@@ -879,6 +923,13 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             __syncwarp();
             if (lane == 0) mbar_arrive(&vfull[b]);
         }
+        if constexpr (SPLIT) {  // the row warps join; what they do in registers these may not have stays theirs
+            __syncthreads();
+            cluster_sync();
+            cluster_sync();
+            __syncthreads();
+            return;
+        }
     } else {
         // ---------------------------------------------------- one row tile
         if constexpr (G::OREG) tc5::setmaxnreg_inc<kChunkRegsRow>();
@@ -888,7 +939,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             const uint64_t f = f0 + (on ? row : 0);
             const uint32_t j = (uint32_t)(f / group), h = kvh * group + (uint32_t)(f - (uint64_t)j * group);
             const uint64_t p = (uint64_t)pos0 + j;
-            const int lim = on && p < a.kv.max_ctx ? (int)p : -1;  // the last position this row sees
+            // the last position this row sees, of this CTA's (none: negative)
+            const int lim = on && p < a.kv.max_ctx ? (int)p - (int)first : -1;
             row_q[row] = (r0 + (uint64_t)j) * a.q.row + (uint64_t)h * a.q.head;
             row_out[row] = (r0 + (uint64_t)j) * a.out.row + (uint64_t)h * a.out.head;
             __syncwarp();
@@ -1132,11 +1184,58 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             // registers of this loop stay its own (rows that see nothing: sums of 0)
             float vunit;
             fit_under(vtop, G::VEXP, &vunit);
-            row_cf[row] = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
+            if constexpr (SPLIT) row_cf[row] = vunit, row_m[row] = mx, row_l[row] = l;
+            else row_cf[row] = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
         }
     }
     __syncwarp();
-    if (warp < 4 * users) {
+    if constexpr (SPLIT) {
+        // Outputs to shared memory, which every product is done with: float4 q of
+        // row r at r * HD / 4 + (q ^ r % 8), elements as below.
+        tc5::fence_before();
+        __syncthreads();
+        tc5::fence_after();
+        float4* rows = reinterpret_cast<float4*>(smem);
+        if (warp < 4 * users) {
+            const uint32_t row = warp * 32 + lane, oc = tmem + G::O_COL + warp / 4 * HD + ((warp % 4 * 32) << 16);
+            const float unit = row_cf[row];
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD / 32; c++) {
+                float y[4][8];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) tc5::ld8(oc + e * (HD / 4) + 8 * c, y[e]);
+                tc5::wait_ld();
+#pragma unroll
+                for (uint32_t q = 0; q < 8; q++)
+                    rows[row * (HD / 4) + ((8 * c + q) ^ (row & 7))] = make_float4(y[0][q] * unit, y[1][q] * unit, y[2][q] * unit, y[3][q] * unit);
+            }
+        }
+        cg::cluster_group cl = cg::this_cluster();
+        cluster_sync();
+        for (uint32_t i = part * 256 + tid; i < live * (HD / 4); i += kKv8ChunkSplits * 256) {
+            const uint32_t row = i / (HD / 4), q = i % (HD / 4);
+            float mm = -INFINITY, ll = 0.0f, mr[kKv8ChunkSplits];
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (uint32_t r = 0; r < kKv8ChunkSplits; r++) {
+                mr[r] = *cl.map_shared_rank(&row_m[row], r);
+                mm = fmaxf(mm, mr[r]);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < kKv8ChunkSplits; r++) {
+                const float f = mr[r] == mm ? 1.0f : ex2(mr[r] - mm);  // (both may be -inf)
+                ll = fmaf(*cl.map_shared_rank(&row_l[row], r), f, ll);
+                const float4 x = *cl.map_shared_rank(&rows[row * (HD / 4) + (q ^ (row & 7))], r);
+                acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
+                acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+            }
+            const float inv = (uint64_t)pos0 + (f0 + row) / group < a.kv.max_ctx ? __frcp_rn(ll) : 0.0f;
+            store4<DT>(const_cast<void*>(a.out.p), row_out[row] + 4 * q, a.out_vec,
+                       make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while others read its rows
+    } else if (warp < 4 * users) {
         // Rows out, 32 columns at a time through the warp's share of q's space:
         // a float4 q of row r lies at r * 8 + (q ^ r % 8). Column e * HD / 4 + i
         // of O' is element 4 i + e. (Every product that reads q is done: the
@@ -1178,8 +1277,27 @@ cudaError_t attend_dt(const Kv8AttendArgs& a, cudaStream_t st) {
     if (a.rows.row_start) {
         using G = ChunkGeom<HD, DT>;
         const uint64_t tiles = (uint64_t)a.rows.n_rows * a.group / G::ROWS + a.rows.n_slots;
-        k_kv8_chunk<HD, DT><<<(uint32_t)(tiles * a.kv.nkv), G::THREADS, G::BYTES, st>>>(a);
-        return cudaGetLastError();
+        k_kv8_chunk<HD, DT, false><<<(uint32_t)(tiles * a.kv.nkv), G::THREADS, G::BYTES, st>>>(a);
+        cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess || !kv8_chunk_shared(1, a.kv.max_ctx - 1, a.kv.nkv)) return e;
+        // Which rows are shared is known on the device only (and must not depend
+        // on the batch): the CTAs set aside for them leave where there are none.
+        Kv8AttendArgs b = a;
+        b.slot_clusters = (uint32_t)std::min<uint64_t>(kKv8ChunkClusters / a.kv.nkv, ((uint64_t)a.rows.n_rows * a.group + G::ROWS - 1) / G::ROWS) * a.kv.nkv;
+        uint64_t clusters = (uint64_t)b.slot_clusters * a.rows.n_slots;
+        if (tiles * a.kv.nkv < clusters) clusters = tiles * a.kv.nkv, b.slot_clusters = 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((uint32_t)clusters * kKv8ChunkSplits);
+        cfg.blockDim = dim3(G::THREADS);
+        cfg.dynamicSmemBytes = G::BYTES;
+        cfg.stream = st;
+        cudaLaunchAttribute attr = {};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = kKv8ChunkSplits;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, k_kv8_chunk<HD, DT, true>, b);
     }
     const bool wide = kv8_single_cols(a.group) == 16;
     cudaLaunchConfig_t cfg = {};
@@ -1202,13 +1320,14 @@ cudaError_t set_limits() {
     cudaError_t e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 1>::RING);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(k_kv8_single<HD, DT, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecGeom<HD, DT, 2>::RING);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(k_kv8_chunk<HD, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkGeom<HD, DT>::BYTES);
-    // what setmaxnreg deals out has to be there
-    cudaFuncAttributes at{};
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, k_kv8_chunk<HD, DT>);
-    if (e == cudaSuccess && ChunkGeom<HD, DT>::OREG && at.numRegs * 3 < 2 * kChunkRegsRow + kChunkRegsCode)
-        e = cudaErrorInvalidConfiguration;
+    for (auto* chunk : {k_kv8_chunk<HD, DT, false>, k_kv8_chunk<HD, DT, true>}) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(chunk, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkGeom<HD, DT>::BYTES);
+        // what setmaxnreg deals out has to be there
+        cudaFuncAttributes at{};
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, chunk);
+        if (e == cudaSuccess && ChunkGeom<HD, DT>::OREG && at.numRegs * 3 < 2 * kChunkRegsRow + kChunkRegsCode)
+            e = cudaErrorInvalidConfiguration;
+    }
     return e;
 }
 

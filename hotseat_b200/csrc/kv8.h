@@ -113,6 +113,18 @@ __host__ __device__ inline uint32_t kv8_split_len(uint32_t n, uint32_t hd, uint3
 // Query heads of one KV head that a CTA takes together.
 constexpr uint32_t kv8_single_cols(uint32_t group) { return group <= 8 ? 8 : 16; }
 
+// Chunks of rows: whether a cluster shares the positions of each tile of 256
+// (row, head) pairs, by the slot's own rows (`tiles` of them, from position
+// pos0 on) and the region's shape alone: where a slot's tiles are few, and for
+// 2,048 positions a CTA at least. 16 rows, 12/2 heads of 128, bf16: 93 us over
+// 32,768 positions (647 by one CTA for each KV head). 64 such slots fill the
+// GPU by themselves and pay for the CTAs' starts and joins: over 9,000
+// positions 328 us shared, 197 not, so shorter ones are left to one CTA.
+constexpr uint32_t kKv8ChunkSplits = 8, kKv8ChunkClusters = 8;  // CTAs of a cluster, clusters of a slot
+__host__ __device__ constexpr bool kv8_chunk_shared(uint64_t tiles, uint32_t pos0, uint32_t nkv) {
+    return tiles * nkv <= kKv8ChunkClusters && pos0 >= 2048 * kKv8ChunkSplits;
+}
+
 // Floats of a cluster's record: outputs, and for each of 8 shares its columns' maxima and sums.
 __host__ __device__ constexpr uint32_t kv8_record(uint32_t hd, uint32_t cols) { return cols * (hd + 16); }
 
@@ -122,6 +134,7 @@ struct Kv8AttendArgs {
     Kv8Mat q, out;
     uint32_t nh = 0, group = 0, chunks = 0;  // query heads, per KV head, and CTAs of kv8_single_cols for these
     float scale = 1.0f;
+    uint32_t slot_clusters = 0;  // split chunks: clusters set aside for each slot; 0: for each tile that the rows can need
     bool q_vec = false, out_vec = false;  // four elements of a row at once: base and strides allow it
     // single rows: CTAs of `cluster` splits join in shared memory; where a
     // region's rows can need more of them, their records [slot][KV head][head

@@ -247,7 +247,7 @@ uint64_t hs_kv8_live_ranges_between(const hs_kv_spec* s, uint32_t block, uint32_
 
 /* n 8-bit regions of one shape, block, page size and device, as the slots of
  * batched calls: the device tables and the workspace of hs_kv8_attend for
- * n_heads query heads (a multiple of the KV heads, at most 16 for each; 0: no
+ * n_heads query heads (a multiple of the KV heads, at most 256 for each; 0: no
  * attend). Like an hs_batch it is used by one call at a time: calls on one
  * set, and replays of graphs captured from them, must follow one another (on
  * one stream, or ordered by events). The regions must outlive it. */
@@ -256,7 +256,8 @@ int hs_kv8_set_new(hs_kv* const* kvs, uint32_t n, uint32_t n_heads, hs_kv8_set**
 void hs_kv8_set_free(hs_kv8_set* s);
 /* Waits for `stream`, then HS_E_ARG if a call since the last check met a row
  * past max_ctx (such rows are not stored, read or attended: outputs of read
- * stay as they were, those of attend are zeros), and clears that. */
+ * stay as they were, those of attend are zeros), HS_E_CUDA if a bounded wait
+ * ran out in one of them (its outputs are not to be used), and clears that. */
 int hs_kv8_set_check(hs_kv8_set* s, void* stream);
 
 /* The calls below enqueue on `stream` (a cudaStream_t of the set's device;
@@ -281,7 +282,8 @@ int hs_kv8_read(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* 
  * region i (so append its K and V first) with its n_heads query heads, query
  * head h on KV head h / (n_heads / n_kv_heads): softmax(scale * q.k) . v.
  * Statistics and sums are f32; a row's bits do not depend on the other slots
- * of the batch. `out` must not overlap `q`. */
+ * of the batch, but on the form (row_start or none) and, with row_start, on
+ * which rows of its own slot the call holds. `out` must not overlap `q`. */
 int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* row_start, const uint32_t* pos,
                   const void* q, uint64_t q_row_stride, uint64_t q_head_stride, void* out, uint64_t out_row_stride,
                   uint64_t out_head_stride, uint32_t dtype, float scale, void* stream);
@@ -385,7 +387,10 @@ int hs_forward_batch(const hs_model* m, hs_kv* const* kvs, const uint32_t* token
  * so the KV rows match single-token steps within the path's tolerance (and
  * are bit-identical however the prompt is cut into calls). Follow
  * with hs_batch_seq_run from filled = pos0 + n: the sequence's next
- * (last prompt) token then produces the logits of the first sample. */
+ * (last prompt) token then produces the logits of the first sample. Over an
+ * 8-bit region what a layer stores depends on how the prompt was cut, within
+ * the path's tolerance: attention's sums there follow the pass's tiles, and
+ * with block > 1 a block's scale is set by the rows that begin it. */
 int hs_prefill(const hs_model* m, hs_kv* kv, const uint32_t* tokens, uint32_t n, uint32_t pos0, hs_batch* b);
 /* Logits of sequence `slot` from the last hs_forward_batch. */
 int hs_batch_logits(hs_batch* b, uint32_t slot, float* host, uint64_t n);

@@ -429,6 +429,51 @@ def test_long_contexts(dtype, hd, nh, nkv, n):
     check_rows(out.float().cpu().numpy()[:1], qf[8:], refs, [(0, n - 1)], hd ** -0.5, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nh, nkv, hd, block, layout", [(14, 2, 64, 1, 0), (12, 2, 128, 32, 1), (5, 1, 128, 1, 0)])
+def test_few_rows_behind_long_contexts(dtype, nh, nkv, hd, block, layout):
+    """Chunks whose positions a cluster shares: slots at and around where it begins, with short and long chunks beside
+    them, one that runs past max_ctx, and each alone with the same bits."""
+    rng = np.random.default_rng(nh * hd)
+    lens, rows = [16387, 16423, 17001, 300, 16385, 17000], [3, 40, 130, 60, 1, 20]
+    kvs, refs = filled(rng, lens, nkv, hd, block, layout)
+    s = hs.Kv8Set(kvs, n_heads=nh)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    pos = [n - m for n, m in zip(lens, rows)]
+    pos[5] += 4  # its last three rows lie past max_ctx (17,001)
+    q, qf = rows_of(rng, sum(rows) + 3, nh, hd, dtype)
+    out = torch.full_like(q, 9.0)
+    s.attend(0, q, out, i32(pos), i32(start))
+    with pytest.raises(hs.HotseatError):
+        s.check()
+    assert bool((out[sum(rows):] == 9.0).all()) and bool((out[sum(rows) - 3:sum(rows)] == 0).all())
+    places = [(i, pos[i] + j) for i, m in enumerate(rows) for j in range(m)]
+    pick = [0, 2, 3, 42, 43, 100, 172, 173, 232, 233, 234, 249]
+    check_rows(out.float().cpu().numpy()[pick], qf[pick], refs, [places[i] for i in pick], hd ** -0.5, dtype)
+    for i, m in enumerate(rows):
+        alone = hs.Kv8Set([kvs[i]], n_heads=nh)
+        part = torch.empty_like(q[:m])
+        alone.attend(0, q[start[i]:start[i + 1]], part, i32([pos[i]]), i32([0, m]))
+        assert torch.equal(part, out[start[i]:start[i + 1]])
+        alone.close()
+
+
+def test_a_shared_chunk_keeps_non_finite_values_apart():
+    """A NaN scale at one position of a split: rows before it do not see it, rows from it on are NaN."""
+    rng = np.random.default_rng(8)
+    kvs, refs = filled(rng, [17000], 2, 64, 1, 0, max_ctx=17100)
+    s = hs.Kv8Set(kvs, n_heads=14)
+    k, _ = rows_of(rng, 10, 2, 64, "f32")
+    k[5] = float("nan")
+    s.append(0, k, k, i32([17000]), i32([0, 10]))
+    for dtype in ("f32", "f16", "bf16"):
+        q, qf = rows_of(rng, 20, 14, 64, dtype)
+        out = torch.empty_like(q)
+        s.attend(0, q, out, i32([16990]), i32([0, 20]))
+        assert bool(out[15:].isnan().all()) and not bool(out[:15].isnan().any())
+        check_rows(out.float().cpu().numpy()[[0, 9]], qf[[0, 9]], refs, [(0, 16990), (0, 16999)], 0.125, dtype)
+
+
 def test_offsets_past_32_bits():
     """A layer behind 4 GiB of others."""
     spec = hs.KvSpec(3, 8, 128, 1 << 20, 1)
