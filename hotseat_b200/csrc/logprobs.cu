@@ -1,24 +1,33 @@
 // Scores of logit rows: log probabilities of given tokens, entropy, rank and
 // the top alternatives, in one pass over the logits.
 //
-// A row is taken by a cluster of up to 8 CTAs, each a contiguous share that
-// its 512 threads hold in registers, so the logits are read once: the
-// maximum, then sum exp(x - m) and sum exp(x - m)(x - m) (for the entropy
-// ln l - t / l), the tokens before the given one, and the top candidates all
-// come from the registers. The CTAs' results meet in distributed shared
-// memory; nothing is kept in global memory between them, so calls on several
-// streams share nothing.
+// A row is cut into up to 8 contiguous shares, taken by a cluster of as many
+// CTAs or, where there are many rows, by fewer in turn (down to one: 2,048 rows
+// of 151,936 in bf16, top 5: 410 us by one CTA a row, 790 by eight: fewer
+// starts, joins and first bounds). The 512 threads of a CTA hold a share in
+// registers, so the logits are read once: the maximum, then sum exp(x - m) and
+// sum exp(x - m)(x - m) (for the entropy ln l - t / l), the tokens before the
+// given one, and the top candidates all come from the registers, while the
+// next share is on its way to the L2. The CTAs' results meet in distributed
+// shared memory; nothing is kept in global memory between them, so calls on
+// several streams share nothing. Shares' sums are joined in one order, whoever
+// took them.
 //
 // Top candidates: the order's key of a token is unique, so the `top`-th
 // largest of the largest keys of 32 or 64 thread groups is a bound that all of
 // a CTA's top tokens reach, and few others: these are collected and each
-// placed by counting the larger ones. Where more tokens reach it than there is
-// room for (logits in order, say), the bound is taken from the threads' own
-// largest keys, which leaves at most 64 x 40. The cluster's first CTA merges
-// the CTAs' lists the same way.
+// placed by counting the larger ones. After a CTA's first share its top tokens
+// so far are such a bound. Where more tokens reach it than there is room for
+// (logits in order, say), the bound is taken from the threads' own largest
+// keys, which leaves at most 64 x 40. The cluster's first CTA merges the CTAs'
+// lists the same way.
 //
-// A row that is longer than a cluster holds (163,840 logits) goes through the
-// registers in strips, their results joined as the CTAs' are.
+// A share that is longer than a CTA holds (20,480 logits) goes through the
+// registers in strips, their results joined in turn.
+//
+// Bound by the instructions of a logit (about a dozen) and the barriers of a
+// strip: 2,048 rows of 151,936 in bf16: entropy alone 300 us (2.1 TB/s), with
+// log probability, rank and 20 alternatives 600. One f32 row: 7.6 and 14 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -119,16 +128,17 @@ __device__ __forceinline__ Sums join_lanes(Sums x, uint32_t n) {
 }
 
 struct Shared {
-    double l[16], t[16];
-    float m[16];
-    uint32_t before[16], n_cand;
+    double l[2][16], t[2][16];     // the warps' sums, of every other strip
+    float m[2][16];
+    uint32_t before[2][16], n_cand[2];
+    float row_m, row_lz;
     uint64_t bound;
     uint64_t group[64];            // largest key of a thread group
     uint64_t best[kThreads];       // ... of a thread (the second way)
     uint64_t cand[kCand];
     uint64_t all[kCluster * kLogprobTop];
-    uint64_t top[kLogprobTop];     // the top tokens so far, in order (0: none)
-    Sums sums[kCluster];           // the first CTA's: every CTA's sums, and top tokens in `all`
+    uint64_t top[2][kLogprobTop];  // the top tokens so far, in order (0: none), and the next ones
+    Sums sums[kCluster];           // the shares' sums; the first CTA's: everyone's, and top tokens in `all`
 };
 
 // Logit i = (j * 512 + tid) * V + e of a strip is this thread's number V j + e.
@@ -138,7 +148,7 @@ __device__ __forceinline__ uint32_t place(uint32_t k) {
 }
 
 template <int DT, int V>
-__global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, uint32_t share) {
+__global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, uint32_t shares, uint32_t share) {
     extern __shared__ __align__(16) uint8_t smem[];
     Shared& s = *reinterpret_cast<Shared*>(smem);
     constexpr uint32_t EB = DT == HS_F32 ? 4 : 2;
@@ -150,14 +160,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
     const uint8_t* row = static_cast<const uint8_t*>(a.logits) + r * a.row_stride * EB;
     const uint32_t id = a.ids ? __ldg(a.ids + r) : 0xffffffffu;
     const float xt = id < a.vocab ? logit<DT>(row, id) : __int_as_float(0x7fc00000);
-    const uint32_t begin = min(rank * share, a.vocab), end = min(begin + share, a.vocab);
     // every CTA of the cluster is there before one writes to the first
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    Sums sums;
-    if (tid < kLogprobTop) s.top[tid] = 0;
+    if (tid < kLogprobTop) s.top[0][tid] = 0;
+    if (tid == 0) s.n_cand[0] = s.n_cand[1] = 0, s.bound = 0;
+    uint32_t cur = 0, strip = 0;  // of s.top and s.n_cand; strips so far
 
-    for (uint32_t from = begin; from < end; from += kStrip) {
-        const uint32_t n = min(kStrip, end - from);
+    for (uint32_t v = rank; v < shares; v += ctas) {
+    const uint32_t begin = min(v * share, a.vocab), end = min(begin + share, a.vocab);
+    if (begin == end && tid == 0) s.sums[v] = Sums();
+    for (uint32_t from = begin; from < end; from += kStrip, strip++) {
+        const uint32_t n = min(kStrip, end - from), par = strip & 1;
         const uint8_t* mine = row + (uint64_t)from * EB;
         // the strip, -inf behind its end
         float x[kPer];
@@ -183,6 +196,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 for (uint32_t e = 0; e < V; e++) x[V * j + e] = i + e < n ? logit<DT>(mine, i + e) : -INFINITY;
             }
         }
+        {   // the next strip on its way to the L2
+            const uint32_t f = from + kStrip < end ? from + kStrip : min((v + ctas) * share, a.vocab);
+            const uint32_t g = v + ctas < shares || f < end ? min(f + min(kStrip, share), a.vocab) : f;
+            for (uint64_t b = tid * 128ull; b < (uint64_t)(g - f) * EB; b += kThreads * 128ull)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(row + (uint64_t)f * EB + b));
+        }
         // the warp's maximum (NaN skipped: it shows in the sums), under which its sums stand
         float m = -INFINITY;
 #pragma unroll
@@ -190,7 +209,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
         const float mine_top = m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (tid == 0) s.n_cand = 0, s.bound = 0;
 
         // Sums over eight logits in f32, over more in f64. A logit 200 below the
         // maximum has no weight, and its distance is cut there: 0 times -inf is not.
@@ -254,9 +272,51 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
             t += __shfl_xor_sync(0xffffffffu, t, o);
             before += __shfl_xor_sync(0xffffffffu, before, o);
         }
-        if (lane == 0) s.l[warp] = l, s.t[warp] = t, s.m[warp] = m, s.before[warp] = before;
+        if (lane == 0) s.l[par][warp] = l, s.t[par][warp] = t, s.m[par][warp] = m, s.before[par][warp] = before;
 
-        if (a.top) {
+        bool all = a.top && strip == 0;  // the same for every thread, as what follows from barriers
+        // Candidates from `bound` on, of a thread that holds any.
+        auto collect = [&](uint64_t bound) {
+            const uint32_t b = (uint32_t)(bound >> 32);
+            // the bound's logit: nothing below it is a candidate
+            const float low = bound == 0 || b == 0xffffffffu ? -INFINITY : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+            bool some = false;
+            if (nan || mine_top >= low) {
+#pragma unroll
+                for (uint32_t k = 0; k < kPer; k++)
+                    if (!(x[k] < low)) {
+                        const uint64_t key = order_key(x[k], from + place<V>(k));
+                        if (place<V>(k) < n && key >= bound) {
+                            const uint32_t c = atomicAdd(&s.n_cand[cur], 1u);
+                            if (c < kCand) s.cand[c] = key;
+                            some = true;
+                        }
+                    }
+            }
+            return some;
+        };
+        if (a.top && strip > 0) {
+            // the top tokens so far are a bound already (the first strip held as many)
+            if (__syncthreads_or(collect(s.top[cur][a.top - 1]))) {
+                const uint32_t nc = s.n_cand[cur];
+                if (nc > kCand) {
+                    all = true;
+                } else {
+                    for (uint32_t i = tid; i < nc + a.top; i += kThreads) {
+                        const uint64_t key = i < nc ? s.cand[i] : s.top[cur][i - nc];
+                        uint32_t above = i < nc ? 0 : i - nc;
+                        for (uint32_t j = 0; j < nc; j++) above += s.cand[j] > key ? 1 : 0;
+                        if (i < nc)
+                            for (uint32_t j = 0; j < a.top; j++) above += s.top[cur][j] > key ? 1 : 0;
+                        if (above < a.top) s.top[cur ^ 1][above] = key;
+                    }
+                    if (tid == 0) s.n_cand[cur ^ 1] = 0;
+                    __syncthreads();
+                    cur ^= 1;
+                }
+            }
+        }
+        if (all) {
             // the thread's largest key: a NaN, else its largest logit, the first of equal ones
             uint32_t at = 0;
 #pragma unroll
@@ -284,6 +344,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
             }
             if (tid % size == 0) s.group[tid / size] = g;
             __syncthreads();
+            // the strips' top tokens so far stand with this one's
+            const uint32_t held = strip > 0 ? a.top : 0;
+            if (tid == 0) s.n_cand[cur] = held, s.bound = 0;
+            if (tid < held) s.cand[tid] = s.top[cur][tid];
+            __syncthreads();
             if (tid < groups) {
                 const uint64_t key = s.group[tid];
                 uint32_t above = 0;
@@ -291,81 +356,68 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 for (uint32_t i = 0; i < groups; i++) above += s.group[i] > key ? 1 : 0;
                 if (key && above == a.top - 1) s.bound = key;
             }
-            if (tid < a.top && s.top[tid]) {  // the strips' so far stand with this one's
-                s.cand[atomicAdd(&s.n_cand, 1u)] = s.top[tid];
-                s.top[tid] = 0;
-            }
             __syncthreads();
-            const uint32_t held = s.n_cand;
-            auto collect = [&](uint64_t bound) {
-                if (best && best >= bound) {
-                    const uint32_t b = (uint32_t)(bound >> 32);
-                    // the bound's logit: nothing below it is a candidate
-                    const float low = bound == 0 || b == 0xffffffffu ? -INFINITY : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-#pragma unroll
-                    for (uint32_t k = 0; k < kPer; k++)
-                        if (!(x[k] < low)) {
-                            const uint64_t key = order_key(x[k], from + place<V>(k));
-                            if (place<V>(k) < n && key >= bound) {
-                                const uint32_t c = atomicAdd(&s.n_cand, 1u);
-                                if (c < kCand) s.cand[c] = key;
-                            }
-                        }
-                }
-            };
-            collect(s.bound);
+            if (best && best >= s.bound) collect(s.bound);
             __syncthreads();
-            if (s.n_cand > kCand) {  // the same for every thread
+            if (s.n_cand[cur] > kCand) {  // the same for every thread
                 s.best[tid] = best;
                 __syncthreads();
-                if (tid == 0) s.n_cand = held, s.bound = 0;
+                if (tid == 0) s.n_cand[cur] = held, s.bound = 0;
                 __syncthreads();
                 uint32_t above = 0;
                 for (uint32_t i = 0; i < kThreads; i++) above += s.best[i] > best ? 1 : 0;
                 if (best && above == a.top - 1) s.bound = best;
                 __syncthreads();
-                collect(s.bound);
+                if (best && best >= s.bound) collect(s.bound);
                 __syncthreads();
             }
-            const uint32_t nc = s.n_cand;
+            const uint32_t nc = s.n_cand[cur];
+            if (tid < a.top) s.top[cur ^ 1][tid] = 0;
+            __syncthreads();
             for (uint32_t i = tid; i < nc; i += kThreads) {
                 const uint64_t key = s.cand[i];
                 uint32_t above = 0;
                 for (uint32_t j = 0; j < nc; j++) above += s.cand[j] > key ? 1 : 0;
-                if (above < a.top) s.top[above] = key;
+                if (above < a.top) s.top[cur ^ 1][above] = key;
             }
+            if (tid == 0) s.n_cand[cur ^ 1] = 0;
+            __syncthreads();
+            cur ^= 1;
         }
-        __syncthreads();
-        // the warps' sums as the CTA's, by the first warp: lanes 0 .. 15, pairs first
-        if (warp == 0) {
-            Sums strip;
+        if (!a.top) __syncthreads();
+        // The warps' sums as the strip's, by one of them: lanes 0 .. 15, pairs
+        // first. (Their places are taken anew two strips on, behind a barrier.)
+        if (warp == strip % (kThreads / 32)) {
+            Sums part;
             if (lane < 16) {
-                strip.l = s.l[lane], strip.t = s.t[lane], strip.m = s.m[lane], strip.before = s.before[lane];
-                if (strip.m == -INFINITY && !isnan(strip.l)) strip.l = strip.t = 0.0;
+                part.l = s.l[par][lane], part.t = s.t[par][lane], part.m = s.m[par][lane], part.before = s.before[par][lane];
+                if (part.m == -INFINITY && !isnan(part.l)) part.l = part.t = 0.0;
             }
-            strip = join_lanes(strip, 16);
-            sums = from == begin ? strip : join(sums, strip);
+            part = join_lanes(part, 16);
+            if (lane == 0) s.sums[v] = from == begin ? part : join(s.sums[v], part);
         }
-        __syncthreads();  // the arrays are free for the next strip
     }
+    }
+    __syncthreads();
     // results go to the cluster's first CTA; the others are done then
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     Shared& to = *cl.map_shared_rank(&s, 0);
     const uint32_t nk = ctas * a.top;
-    if (tid == 0) to.sums[rank] = sums;
-    if (tid < a.top) to.all[rank * a.top + tid] = s.top[tid];
+    if (rank > 0 && tid < shares && tid % ctas == rank) to.sums[tid] = s.sums[tid];
+    if (tid < a.top) to.all[rank * a.top + tid] = s.top[cur][tid];
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (rank != 0) return;
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (warp == 0) {
-        if (lane < ctas) sums = s.sums[lane];
-        sums = join_lanes(sums, ctas);
+        Sums sums;
+        if (lane < shares) sums = s.sums[lane];
+        sums = join_lanes(sums, shares);
         // nothing but -inf, or +inf: no distribution
         if (sums.m == -INFINITY || sums.m == INFINITY) sums.l = sums.t = __longlong_as_double(0x7ff8000000000000ll);
         const double lz = log(sums.l);
         if (lane == 0) {
-            s.m[0] = sums.m;
-            s.m[1] = (float)lz;
+            s.row_m = sums.m;
+            s.row_lz = (float)lz;
             if (a.logp) a.logp[r] = (xt - sums.m) - (float)lz;
             if (a.entropy) a.entropy[r] = (float)(lz - sums.t / sums.l);
             if (a.rank) a.rank[r] = id < a.vocab ? sums.before : 0xffffffffu;
@@ -381,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
         if (above < a.top) {
             const uint32_t tok = key_id(key);
             if (a.top_ids) a.top_ids[r * a.top + above] = tok;
-            if (a.top_logp) a.top_logp[r * a.top + above] = (logit<DT>(row, tok) - s.m[0]) - s.m[1];
+            if (a.top_logp) a.top_logp[r * a.top + above] = (logit<DT>(row, tok) - s.row_m) - s.row_lz;
         }
     }
 }
@@ -391,9 +443,13 @@ cudaError_t launch_dt(const LogprobArgs& a, cudaStream_t st) {
     // Shares of a multiple of 8 logits, so that they start as aligned as the row
     // does; a short row's are 4,096 logits at least.
     constexpr int V = DT == HS_F32 ? 4 : 8;
+    uint32_t shares = 1;
+    while (shares < kCluster && shares * 4096u < a.vocab) shares *= 2;
+    const uint32_t share = ((a.vocab + shares - 1) / shares + 7) / 8 * 8;
+    // Few rows: a CTA a share. Rows that fill the GPU's 296 places twice without
+    // that: fewer CTAs a row, which take its shares in turn, with the same sums.
     uint32_t ctas = 1;
-    while (ctas < kCluster && ctas * 4096u < a.vocab) ctas *= 2;
-    const uint32_t share = ((a.vocab + ctas - 1) / ctas + 7) / 8 * 8;
+    while (ctas < shares && (uint64_t)a.rows * ctas < 4 * 148) ctas *= 2;
     const uint64_t bytes = DT == HS_F32 ? 4 : 2;
     const bool vec = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride * bytes % 16 == 0;
     cudaLaunchConfig_t cfg = {};
@@ -408,7 +464,7 @@ cudaError_t launch_dt(const LogprobArgs& a, cudaStream_t st) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return vec ? cudaLaunchKernelEx(&cfg, k_logprobs<DT, V>, a, share) : cudaLaunchKernelEx(&cfg, k_logprobs<DT, 1>, a, share);
+    return vec ? cudaLaunchKernelEx(&cfg, k_logprobs<DT, V>, a, shares, share) : cudaLaunchKernelEx(&cfg, k_logprobs<DT, 1>, a, shares, share);
 }
 
 }  // namespace

@@ -157,6 +157,35 @@ def test_a_rows_bits_do_not_depend_on_the_batch_or_the_call():
     assert np.array_equal(out.cpu().numpy(), a["logp"])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab, top", [(9001, 64), (70003, 5), (200011, 20)])
+def test_many_rows_have_the_bits_of_few(dtype, vocab, top):
+    """Up to 600 rows at once against the same rows in calls of 12: plain ones, logits in order either way, ties, masked
+    rows with and without enough tokens left, NaN."""
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    some = torch.randn(12, vocab, generator=g, device="cuda") * 3
+    some[1] = torch.arange(vocab, device="cuda") / vocab * 8
+    some[2] = -some[1]
+    some[3] = torch.randint(-2, 3, (vocab,), generator=g, device="cuda").float()
+    some[4, :-3] = -inf
+    some[5] = -inf
+    some[6, 100:-100] = -inf
+    some[7, -1] = nan
+    some[8, ::2] = nan
+    some[9, vocab // 2] = inf
+    some[10, vocab // 2:] += 20.0
+    some = some.to(DT[dtype])
+    ids = torch.tensor([0, 5, vocab - 1, 77, vocab - 2, 3, 50, 9, 11, 4, vocab - 1, -1], dtype=torch.int32, device="cuda")
+    check(some, ids, top)
+    few = run(some, ids, top)
+    for times in (50, 26, 13):
+        many = run(some.repeat(times, 1), ids.repeat(times), top)
+        for k in few:
+            want = np.tile(few[k], (times,) + (1,) * (few[k].ndim - 1))
+            assert np.array_equal(many[k], want, equal_nan=want.dtype == np.float32), (k, times)
+
+
 def test_scores_of_a_forward(tiny_gguf):
     m = hs.Model.load(tiny_gguf, max_ctx=16)
     s, kv = m.scratch(), m.kv()
