@@ -13,6 +13,12 @@ Rust API that hotseat's worker calls on hs-engine (crates/hs-engine/src):
     argmax(s)                         sampler.rs:177 argmax
     run_seq(...)                      hs-worker seq.rs:230 run
 
+and, without a counterpart there:
+
+    Kv.alloc8(spec, block) / model.kv8(...)   a cache in int8 codes
+    Kv8Set(kvs, n_heads).append/read/attend   batched rows of such caches (device memory)
+    logprobs(logits, ids, ...)                log probabilities, entropy, rank, top tokens
+
 All compute runs in libhotseat.so on the GPU. There is no CPU fallback: if the
 library is missing the import fails, and a call without a GPU raises.
 """

@@ -116,13 +116,13 @@ constexpr uint32_t kv8_single_cols(uint32_t group) { return group <= 8 ? 8 : 16;
 // Chunks of rows: whether a cluster shares the positions of each tile of 256
 // (row, head) pairs, by the slot's own rows (`tiles` of them, from position
 // pos0 on) and the region's shape alone: where a slot's tiles are few, and for
-// 2,048 positions a CTA at least. 16 rows, 12/2 heads of 128, bf16: 93 us over
-// 32,768 positions (647 by one CTA for each KV head). 64 such slots fill the
-// GPU by themselves and pay for the CTAs' starts and joins: over 9,000
-// positions 328 us shared, 197 not, so shorter ones are left to one CTA.
+// 512 positions a CTA at least. 16 rows a slot, 12/2 heads of 128, bf16, over
+// 5,000 positions: 25 us shared, 110 by one CTA for each KV head; 16 such slots
+// 72 and 112; 64 slots, which fill the GPU by themselves and pay for the CTAs'
+// starts and joins, 234 and 117. One slot over 32,768 positions: 93 and 647.
 constexpr uint32_t kKv8ChunkSplits = 8, kKv8ChunkClusters = 8;  // CTAs of a cluster, clusters of a slot
 __host__ __device__ constexpr bool kv8_chunk_shared(uint64_t tiles, uint32_t pos0, uint32_t nkv) {
-    return tiles * nkv <= kKv8ChunkClusters && pos0 >= 2048 * kKv8ChunkSplits;
+    return tiles * nkv <= kKv8ChunkClusters && pos0 >= 512 * kKv8ChunkSplits;
 }
 
 // Floats of a cluster's record: outputs, and for each of 8 shares its columns' maxima and sums.

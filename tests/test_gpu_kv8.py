@@ -435,12 +435,12 @@ def test_few_rows_behind_long_contexts(dtype, nh, nkv, hd, block, layout):
     """Chunks whose positions a cluster shares: slots at and around where it begins, with short and long chunks beside
     them, one that runs past max_ctx, and each alone with the same bits."""
     rng = np.random.default_rng(nh * hd)
-    lens, rows = [16387, 16423, 17001, 300, 16385, 17000], [3, 40, 130, 60, 1, 20]
+    lens, rows = [4099, 4135, 9001, 300, 4097, 9000], [3, 40, 130, 60, 1, 20]
     kvs, refs = filled(rng, lens, nkv, hd, block, layout)
     s = hs.Kv8Set(kvs, n_heads=nh)
     start = np.concatenate([[0], np.cumsum(rows)])
     pos = [n - m for n, m in zip(lens, rows)]
-    pos[5] += 4  # its last three rows lie past max_ctx (17,001)
+    pos[5] += 4  # its last three rows lie past max_ctx (9,001)
     q, qf = rows_of(rng, sum(rows) + 3, nh, hd, dtype)
     out = torch.full_like(q, 9.0)
     s.attend(0, q, out, i32(pos), i32(start))
@@ -461,17 +461,17 @@ def test_few_rows_behind_long_contexts(dtype, nh, nkv, hd, block, layout):
 def test_a_shared_chunk_keeps_non_finite_values_apart():
     """A NaN scale at one position of a split: rows before it do not see it, rows from it on are NaN."""
     rng = np.random.default_rng(8)
-    kvs, refs = filled(rng, [17000], 2, 64, 1, 0, max_ctx=17100)
+    kvs, refs = filled(rng, [9000], 2, 64, 1, 0, max_ctx=9100)
     s = hs.Kv8Set(kvs, n_heads=14)
     k, _ = rows_of(rng, 10, 2, 64, "f32")
     k[5] = float("nan")
-    s.append(0, k, k, i32([17000]), i32([0, 10]))
+    s.append(0, k, k, i32([9000]), i32([0, 10]))
     for dtype in ("f32", "f16", "bf16"):
         q, qf = rows_of(rng, 20, 14, 64, dtype)
         out = torch.empty_like(q)
-        s.attend(0, q, out, i32([16990]), i32([0, 20]))
+        s.attend(0, q, out, i32([8990]), i32([0, 20]))
         assert bool(out[15:].isnan().all()) and not bool(out[:15].isnan().any())
-        check_rows(out.float().cpu().numpy()[[0, 9]], qf[[0, 9]], refs, [(0, 16990), (0, 16999)], 0.125, dtype)
+        check_rows(out.float().cpu().numpy()[[0, 9]], qf[[0, 9]], refs, [(0, 8990), (0, 8999)], 0.125, dtype)
 
 
 def test_offsets_past_32_bits():
