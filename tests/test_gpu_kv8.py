@@ -456,6 +456,22 @@ def test_few_rows_behind_long_contexts(dtype, nh, nkv, hd, block, layout):
         alone.attend(0, q[start[i]:start[i + 1]], part, i32([pos[i]]), i32([0, m]))
         assert torch.equal(part, out[start[i]:start[i + 1]])
         alone.close()
+    # captured, on another stream, and beside a call on another set
+    side, first = torch.cuda.Stream(), out.clone()
+    start_d, pos_d = i32(start), i32(pos)
+    twin, out2 = hs.Kv8Set(kvs[:1], n_heads=nh), torch.empty_like(q[:3])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        s.attend(0, q, out, pos_d, start_d, stream=side.cuda_stream)
+    for _ in range(3):
+        out.fill_(9.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        twin.attend(0, q[:3], out2, i32(pos[:1]), i32([0, 3]))
+        torch.cuda.synchronize()
+        assert torch.equal(out, first) and torch.equal(out2, first[:3])
 
 
 def test_a_shared_chunk_keeps_non_finite_values_apart():
