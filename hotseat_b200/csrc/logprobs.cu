@@ -275,29 +275,37 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
         if (lane == 0) s.l[par][warp] = l, s.t[par][warp] = t, s.m[par][warp] = m, s.before[par][warp] = before;
 
         bool all = a.top && strip == 0;  // the same for every thread, as what follows from barriers
-        // Candidates from `bound` on, of a thread that holds any.
-        auto collect = [&](uint64_t bound) {
-            const uint32_t b = (uint32_t)(bound >> 32);
-            // the bound's logit: nothing below it is a candidate
-            const float low = bound == 0 || b == 0xffffffffu ? -INFINITY : __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-            bool some = false;
-            if (nan || mine_top >= low) {
+        // Candidates from `bound` on, of the threads that may hold any: few, so that
+        // their warp reads their logits again, eight lanes a thread's (a thread over
+        // its own registers is 40 steps of code that the others wait for).
+        auto collect = [&](bool holds, uint64_t bound) {
+            const uint32_t all_of = __ballot_sync(0xffffffffu, holds);
+            for (uint32_t who = all_of; who;) {
+                uint32_t one = who;  // without its first lane / 8
 #pragma unroll
-                for (uint32_t k = 0; k < kPer; k++)
-                    if (!(x[k] < low)) {
-                        const uint64_t key = order_key(x[k], from + place<V>(k));
-                        if (place<V>(k) < n && key >= bound) {
-                            const uint32_t c = atomicAdd(&s.n_cand[cur], 1u);
-                            if (c < kCand) s.cand[c] = key;
-                            some = true;
-                        }
+                for (uint32_t i = 0; i < 4; i++) {
+                    if (i < lane / 8) one &= one - 1;
+                    who &= who - 1;
+                }
+                if (!one) continue;
+                const uint32_t t = warp * 32 + __ffs(one) - 1;
+#pragma unroll
+                for (uint32_t i = 0; i < kPer / 8; i++) {
+                    const uint32_t k = 8 * i + lane % 8, p = (k / V * kThreads + t) * V + k % V;
+                    if (p >= n) continue;
+                    const uint64_t key = order_key(logit<DT>(mine, p), from + p);
+                    if (key >= bound) {
+                        const uint32_t c = atomicAdd(&s.n_cand[cur], 1u);
+                        if (c < kCand) s.cand[c] = key;
                     }
+                }
             }
-            return some;
+            return all_of != 0;
         };
         if (a.top && strip > 0) {
             // the top tokens so far are a bound already (the first strip held as many)
-            if (__syncthreads_or(collect(s.top[cur][a.top - 1]))) {
+            const uint64_t bound = s.top[cur][a.top - 1];
+            if (__syncthreads_or(collect(nan || order_key(mine_top, from + place<V>(0)) >= bound, bound))) {
                 const uint32_t nc = s.n_cand[cur];
                 if (nc > kCand) {
                     all = true;
@@ -324,15 +332,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 const uint32_t k = kPer - 1 - i;
                 if (x[k] == mine_top) at = k;
             }
-            uint64_t best = 0;
-            if (nan || mine_top == -INFINITY) {
-#pragma unroll
+            uint64_t best = place<V>(at) < n ? order_key(mine_top, from + place<V>(at)) : 0;
+            if (nan) {
+#pragma unroll 1
                 for (uint32_t k = 0; k < kPer; k++) {
-                    const uint64_t key = order_key(x[k], from + place<V>(k));
-                    if (place<V>(k) < n && key > best) best = key;
+                    if (place<V>(k) >= n) continue;
+                    const uint64_t key = order_key(logit<DT>(mine, place<V>(k)), from + place<V>(k));
+                    if (key > best) best = key;
                 }
-            } else {
-                best = order_key(mine_top, from + place<V>(at));
             }
             // groups of 16 threads, of 8 for more than 16 tokens; the bound is the
             // key that top - 1 of theirs are above (0 if fewer hold any)
@@ -357,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 if (key && above == a.top - 1) s.bound = key;
             }
             __syncthreads();
-            if (best && best >= s.bound) collect(s.bound);
+            collect(best && best >= s.bound, s.bound);
             __syncthreads();
             if (s.n_cand[cur] > kCand) {  // the same for every thread
                 s.best[tid] = best;
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
                 for (uint32_t i = 0; i < kThreads; i++) above += s.best[i] > best ? 1 : 0;
                 if (best && above == a.top - 1) s.bound = best;
                 __syncthreads();
-                if (best && best >= s.bound) collect(s.bound);
+                collect(best && best >= s.bound, s.bound);
                 __syncthreads();
             }
             const uint32_t nc = s.n_cand[cur];
