@@ -3,8 +3,8 @@
 //
 // A row is cut into up to 8 contiguous shares, taken by a cluster of as many
 // CTAs or, where there are many rows, by fewer in turn (down to one: 2,048 rows
-// of 151,936 in bf16, all outputs, top 5: 521 us by one CTA a row, 790 by eight:
-// fewer starts, joins and first bounds). The 512 threads of a CTA hold a share in
+// of 151,936 in bf16, all outputs, top 5: 400 us; one CTA a row instead of eight,
+// so fewer starts, joins and first bounds, was 790 -> 521 of that). The 512 threads of a CTA hold a share in
 // registers, so the logits are read once: the maximum, then sum exp(x - m) and
 // sum exp(x - m)(x - m) (for the entropy ln l - t / l), the tokens before the
 // given one, and the top candidates all come from the registers, while the
@@ -26,8 +26,8 @@
 // registers in strips, their results joined in turn.
 //
 // Bound by the instructions of a logit (about a dozen) and the barriers of a
-// strip: 2,048 rows of 151,936 in bf16: entropy alone 300 us (2.1 TB/s), with
-// log probability, rank and 20 alternatives 600. One f32 row: 7.6 and 14 us.
+// strip: 2,048 rows of 151,936 in bf16: entropy alone 294 us (2.1 TB/s), with
+// log probability, rank and 20 alternatives 443. One f32 row: 7.6 and 12.9 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
