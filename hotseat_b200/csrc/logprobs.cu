@@ -3,9 +3,10 @@
 //
 // A row is cut into up to 8 contiguous shares, taken by a cluster of as many
 // CTAs or, where there are many rows, by fewer in turn (down to one: 2,048 rows
-// of 151,936 in bf16, all outputs, top 5: 400 us; one CTA a row instead of eight,
-// so fewer starts, joins and first bounds, was 790 -> 521 of that). The 512 threads of a CTA hold a share in
-// registers, so the logits are read once: the maximum, then sum exp(x - m) and
+// of 151,936 in bf16, all outputs, top 5: 400 us; one CTA a row instead of
+// eight, so fewer starts, joins and first bounds, was 790 -> 521 of that). The
+// 512 threads of a CTA hold a share in registers, so the logits are read once
+// (but for the candidates): the maximum, then sum exp(x - m) and
 // sum exp(x - m)(x - m) (for the entropy ln l - t / l), the tokens before the
 // given one, and the top candidates all come from the registers, while the
 // next share is on its way to the L2. The CTAs' results meet in distributed

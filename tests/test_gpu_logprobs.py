@@ -186,6 +186,19 @@ def test_many_rows_have_the_bits_of_few(dtype, vocab, top):
             assert np.array_equal(many[k], want, equal_nan=want.dtype == np.float32), (k, times)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_many_rows_off_their_alignment(dtype):
+    """Rows that begin one element past an aligned place, in one call of 600 and in small ones."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn(600, 9003, generator=g, device="cuda") * 4).to(DT[dtype])[:, 1:]
+    ids = torch.randint(0, 9002, (600,), generator=g, device="cuda", dtype=torch.int32)
+    many = run(x, ids, 33)
+    check(x[590:], ids[590:], 33)
+    for at in (0, 299, 590):
+        few = run(x[at:at + 10], ids[at:at + 10], 33)
+        assert all(np.array_equal(many[k][at:at + 10], few[k]) for k in few)
+
+
 def test_scores_of_a_forward(tiny_gguf):
     m = hs.Model.load(tiny_gguf, max_ctx=16)
     s, kv = m.scratch(), m.kv()
