@@ -487,8 +487,10 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
         return;
     }
 
-    // a cluster's splits: CTA `rank` joins its share of the outputs
+    // a cluster's splits: CTA `rank` joins its share of the outputs (the lanes'
+    // loops before a cluster's barrier differ in length, and a warp meets it as one)
     cg::cluster_group cl = cg::this_cluster();
+    __syncwarp();
     cl.sync();
     const uint32_t rank = split - first, held = min(cs, splits - first);
     const uint32_t shares = splits <= cs ? splits : cs;
@@ -525,6 +527,7 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
         }
     }
     // no CTA leaves while others read its record
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
     if (n_cl == 1) return;
 
@@ -775,6 +778,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             dead = true;
             atomicOr(a.rows.err, ERR_TIMEOUT);
         }
+        __syncwarp();  // lanes leave the loop apart, and warp-wide instructions follow
     };
 
     if (warp >= 8) {

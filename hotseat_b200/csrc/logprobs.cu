@@ -413,6 +413,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_logprobs(const LogprobArgs a, u
     const uint32_t nk = ctas * a.top;
     if (rank > 0 && tid < shares && tid % ctas == rank) to.sums[tid] = s.sums[tid];
     if (tid < a.top) to.all[rank * a.top + tid] = s.top[cur][tid];
+    __syncwarp();  // the barrier takes a warp as one
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     if (rank != 0) return;
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");

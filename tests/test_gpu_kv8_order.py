@@ -1,0 +1,48 @@
+"""Order between threads, products and kernels of the 8-bit cache and the
+logit scores: calls whose warps, tiles or clusters finish apart give the same
+bits every time, and the right ones."""
+import numpy as np
+import pytest
+
+import hotseat_b200 as hs
+from test_gpu_kv8 import check_rows, filled, i32, rows_of
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("nh, nkv, hd, n", [(14, 2, 64, 2048), (7, 1, 64, 1300), (5, 1, 128, 1100), (12, 2, 128, 20000)])
+def test_single_rows_whose_shares_leave_lanes_idle(dtype, nh, nkv, hd, n):
+    """A cluster's share of the outputs is no multiple of a warp: 7 columns of 64 in 8 shares are 14 pieces each."""
+    rng = np.random.default_rng(n)
+    kvs, refs = filled(rng, [n, n - 500], nkv, hd, 1, 0)
+    s = hs.Kv8Set(kvs, n_heads=nh)
+    q, qf = rows_of(rng, 2, nh, hd, dtype)
+    pos, first = i32([n - 1, n - 501]), None
+    for _ in range(40):
+        out = torch.full_like(q, 9.0)
+        s.attend(0, q, out, pos)
+        first = out if first is None else first
+        assert torch.equal(out, first)
+    check_rows(first.float().cpu().numpy(), qf, refs, [(0, n - 1), (1, n - 501)], hd ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("rows, vocab, top", [(1, 151936, 5), (3, 40000, 20), (40, 20000, 3), (80, 9000, 64)])
+def test_logit_scores_of_a_cluster_repeat(rows, vocab, top):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, vocab, generator=g, device="cuda") * 3
+    ids = torch.randint(0, vocab, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    first = None
+    for _ in range(40):
+        o = dict(logp=torch.empty(rows, device="cuda"), entropy=torch.empty(rows, device="cuda"),
+                 rank=torch.empty(rows, dtype=torch.int32, device="cuda"),
+                 top_ids=torch.empty(rows, top, dtype=torch.int32, device="cuda"),
+                 top_logp=torch.empty(rows, top, device="cuda"))
+        hs.logprobs(x, ids, **o)
+        first = first or o
+        assert all(torch.equal(o[k], first[k]) for k in o)
+    want = torch.log_softmax(x.double(), -1).gather(1, ids.long()[:, None])[:, 0]
+    assert float((first["logp"] - want).abs().max()) <= 64 * 2.0 ** -24 * float(want.abs().max())
+    assert torch.equal(first["top_ids"].long(), torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top])
