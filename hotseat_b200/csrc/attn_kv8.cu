@@ -577,7 +577,8 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 //   S = Q K^T    A = Q (shared), B = K (shared), 128 x 128
 //   O' = W V     A = W (TMEM),   B = V^T (shared), 128 x head_dim
 //
-// While one row tile's threads are at their softmax the other's products run.
+// While one row tile's threads are at their softmax the other's products run;
+// a tile's own follow one another, as its next scores take its weights' place.
 //
 // SPLIT: few rows over many positions (kv8_chunk_shared), which would leave
 // most SMs idle. A cluster's CTAs take the positions in equal runs of steps,
@@ -1172,7 +1173,12 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                 bar_sync(1 + w);
                 if (issuer) {
                     issue_o(t);
-                    if (t + 1 < tiles) issue_s(t + 1);
+                    // The next scores go where this tile's weights lie, and products with
+                    // different accumulators are not bound to run in the order of their issue.
+                    if (t + 1 < tiles) {
+                        wait(&o_done[w], t & 1);
+                        issue_s(t + 1);
+                    }
                 }
             }
             if constexpr (G::OREG) {  // their sums back where the last tile's were

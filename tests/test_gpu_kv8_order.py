@@ -46,3 +46,26 @@ def test_logit_scores_of_a_cluster_repeat(rows, vocab, top):
     want = torch.log_softmax(x.double(), -1).gather(1, ids.long()[:, None])[:, 0]
     assert float((first["logp"] - want).abs().max()) <= 64 * 2.0 ** -24 * float(want.abs().max())
     assert torch.equal(first["top_ids"].long(), torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :top])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nh, nkv, hd, block", [(14, 2, 64, 16), (12, 2, 128, 1)])
+def test_chunks_repeat_over_many_tiles(dtype, nh, nkv, hd, block):
+    """Prompts, one row tile alone and rows that a cluster shares: each tile's scores take the place of the weights
+    that the product before them read."""
+    rng = np.random.default_rng(hd)
+    lens, rows = [1500, 2000, 700, 5000], [300, 40, 700, 9]
+    kvs, refs = filled(rng, lens, nkv, hd, block, 0)
+    s = hs.Kv8Set(kvs, n_heads=nh)
+    start = np.concatenate([[0], np.cumsum(rows)])
+    q, qf = rows_of(rng, sum(rows), nh, hd, dtype)
+    pos, start_d, first = i32([n - m for n, m in zip(lens, rows)]), i32(start), None
+    for _ in range(20):
+        out = torch.full_like(q, 9.0)
+        s.attend(0, q, out, pos, start_d)
+        first = out if first is None else first
+        assert torch.equal(out, first)
+    s.check()
+    places = [(i, n - m + j) for i, (n, m) in enumerate(zip(lens, rows)) for j in range(m)]
+    pick = [0, 299, 300, 339, 340, 700, 1039, 1040, 1048]
+    check_rows(first.float().cpu().numpy()[pick], qf[pick], refs, [places[i] for i in pick], hd ** -0.5, dtype)
