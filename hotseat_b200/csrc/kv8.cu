@@ -147,8 +147,10 @@ __device__ __forceinline__ void values8(uint2 c, float s, float* x) {
         x[e] = __fmul_rn(__fsub_rn(__uint_as_float(__byte_perm(w[e >> 2], 0x4b000000u, 0x7440 | (e & 3))), 8388736.0f), s);
 }
 
-// Sets the page bits of `len` bytes at `off`, after they are visible (a
-// harvest may run concurrently).
+// Sets the page bits of `len` bytes at `off`. A harvest and an arm may run
+// concurrently, so a warp that stored rows first fences, then reads whether the
+// region is tracked (an arm that this read misses comes after the stores, and so
+// do the copies behind it), then meets its other lanes, then marks.
 __device__ __forceinline__ void mark_pages(const Kv8View& kv, uint32_t slot, uint64_t off, uint32_t len) {
     uint64_t* dirty = kv.dirty[slot];
     for (uint64_t pg = off >> kv.page_shift; pg <= (off + len - 1) >> kv.page_shift; pg++)
@@ -271,9 +273,9 @@ __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, cons
                     if (p.e == 0) *reinterpret_cast<float*>(scale) = s;
                 }
         }
+        __threadfence();
+        __syncwarp();
         if (tracked(kv, walk.slot)) {
-            __threadfence();
-            __syncwarp();
             for (uint32_t h = lane; h < 2 * kv.nkv * n; h += 32) {
                 const uint32_t i = h / (2 * kv.nkv), w = h / kv.nkv & 1, head = h % kv.nkv;
                 mark_pages(kv, walk.slot, kv.code_off(w, head, pos + i), HD);
@@ -355,8 +357,10 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
     float s = scale_for(top), held = 0.0f;
     int k2 = 0;
     if (live && b0 < p0) held = *reinterpret_cast<const float*>(base + sat);
-    if (WPU > 1) __syncthreads();  // every warp holds the old scale before one writes the new one
-    if (!live) return;
+    // every thread of the unit holds the old scale before one writes the new one
+    if (WPU > 1) __syncthreads();
+    else __syncwarp();
+    if (!live) return;  // the whole unit
     if (isnan(held)) {
         s = held;
     } else if (held > 0.0f && !isnan(s)) {
@@ -364,11 +368,12 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
         s = __fmul_rn(__fmul_rn(held, pow2i(k2 / 2)), pow2i(k2 - k2 / 2));  // 2^k2 itself may pass f32
     }
     const float inv = s > 0.0f ? reciprocal(s) : 0.0f;
-    const bool track = tracked(kv, slot);
+    // new rows, and older ones where the scale grew
+    auto stored = [&](uint64_t p) { return p < end && p < kv.max_ctx && (p >= p0 || k2 > 0); };
 #pragma unroll
     for (uint32_t i = 0; i < RL; i++) {
         const uint64_t p = b0 + j0 + i * WPU * RPW;
-        if (p >= end || p >= kv.max_ctx || (p < p0 && k2 == 0)) continue;
+        if (!stored(p)) continue;
         const uint64_t at = kv.code_off(is_v, head, (uint32_t)p);
         uint2* to = reinterpret_cast<uint2*>(base + at + 8 * tl);
         uint2 c = make_uint2(0, 0);
@@ -386,18 +391,17 @@ __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, co
             c = make_uint2(n[0], n[1]);
         }
         *to = c;
-        if (track) {
-            __threadfence();
-            if (tl == 0) mark_pages(kv, slot, at, HD);
-        }
     }
-    if (j0 == 0 && tl == 0) {
-        *reinterpret_cast<float*>(base + sat) = s;
-        if (track) {
-            __threadfence();
-            mark_pages(kv, slot, sat, 4);
-        }
+    if (j0 == 0 && tl == 0) *reinterpret_cast<float*>(base + sat) = s;
+    __threadfence();
+    __syncwarp();
+    if (tl != 0 || !tracked(kv, slot)) return;
+#pragma unroll 1
+    for (uint32_t i = 0; i < RL; i++) {
+        const uint64_t p = b0 + j0 + i * WPU * RPW;
+        if (stored(p)) mark_pages(kv, slot, kv.code_off(is_v, head, (uint32_t)p), HD);
     }
+    if (j0 == 0) mark_pages(kv, slot, sat, 4);
 }
 
 // Read back: as k_append_rows, four rows' pieces in flight at once; bound by

@@ -69,3 +69,46 @@ def test_chunks_repeat_over_many_tiles(dtype, nh, nkv, hd, block):
     places = [(i, n - m + j) for i, (n, m) in enumerate(zip(lens, rows)) for j in range(m)]
     pick = [0, 299, 300, 339, 340, 700, 1039, 1040, 1048]
     check_rows(first.float().cpu().numpy()[pick], qf[pick], refs, [places[i] for i in pick], hd ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("block, layout, hd", [(1, 0, 64), (16, 0, 64), (16, 1, 128), (64, 1, 64), (128, 0, 128)])
+def test_a_pre_copy_beside_appends_misses_nothing(block, layout, hd):
+    """Armed, harvested and copied while appends run on another stream: once these are done, one more harvest makes
+    the copy equal. Half steps keep a row's lanes apart."""
+    rng = np.random.default_rng(block)
+    spec = hs.KvSpec(1, 2, hd, 1024, layout)
+    src, dst = hs.Kv.alloc8(spec, block=block, page_size=256), hs.Kv.alloc8(spec, block=block, page_size=256)
+    s, side = hs.Kv8Set([src]), torch.cuda.Stream()
+    x = rng.integers(-126, 126, (1024, 2, hd)) + np.where(rng.random((1024, 2, hd)) < 0.1, 0.5, 0.0)
+    x[..., 0] = 127.0
+    x = x * 2.0 ** rng.integers(0, 3, (1024, 1, 1))
+    k = torch.from_numpy(x.astype(np.float32)).cuda()
+    starts, sizes = [], []
+    p = 0
+    while p < 1024:
+        m = min(int(rng.integers(1, 9)), 1024 - p)
+        starts.append(i32([p]))
+        sizes.append((p, m, i32([0, m])))
+        p += m
+    torch.cuda.synchronize()
+    at = 0
+
+    def some(n):
+        nonlocal at
+        for pos, (p, m, row) in zip(starts[at:at + n], sizes[at:at + n]):
+            s.append(0, k[p:p + m], k[p:p + m], pos, row, stream=side.cuda_stream)
+        at += n
+
+    whole = [(0, src.bytes)]
+    some(20)
+    src.arm()
+    src.copy_runs_to(dst, whole)
+    while at < len(starts):
+        some(12)
+        words = src.harvest()
+        src.copy_runs_to(dst, hs.runs_to_byte_runs(words, src.n_pages, src.page_size, whole))
+    side.synchronize()
+    src.copy_runs_to(dst, hs.runs_to_byte_runs(src.harvest(), src.n_pages, src.page_size, whole))
+    assert np.array_equal(src.read(0, src.bytes), dst.read(0, dst.bytes))
+    src.disarm()
+    s.check()
