@@ -177,9 +177,10 @@ struct DecGeom {
     static constexpr uint32_t RING = W * STAGES * STAGE;
     static constexpr uint32_t OS = HD + 4;  // row stride of the outputs, which take the ring's space
     static_assert(RING >= W * NC * OS * 4, "the outputs fit in the ring");
-    // f32 rows keep q and the weights as pairs; f16 ones the weights (one f16
-    // would double their result's own rounding); q of 16 bits is exact in one
-    static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
+    // f32 rows keep q as pairs; q of 16 bits is exact in one f16. Weights are
+    // pairs for every type: one f16 moves a result by 2^-12 of the largest value
+    // under it, which a sum of values that cancel shows in bf16 too.
+    static constexpr bool QPAIR = DT == HS_F32;
 };
 
 template <int HD, int DT, int NT>
@@ -420,14 +421,14 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
                     l[nt][e & 1] += p;
                     w[e] = p * (vs[b][e >> 1] * vfit);
                 }
-                uint32_t w0, w1, x0 = 0, x1 = 0;
+                uint32_t w0, w1, x0, x1;
                 pair16(w[0], w[1], &w0, &x0);
                 pair16(w[2], w[3], &w1, &x1);
                 w0 = transpose8x8(w0), w1 = transpose8x8(w1);
-                if constexpr (G::WPAIR) x0 = transpose8x8(x0), x1 = transpose8x8(x1);
+                x0 = transpose8x8(x0), x1 = transpose8x8(x1);
 #pragma unroll
                 for (uint32_t i = 0; i < KS; i++) {
-                    if constexpr (G::WPAIR) mma16816(o[nt][i], va[b][i], x0, x1);
+                    mma16816(o[nt][i], va[b][i], x0, x1);
                     mma16816(o[nt][i], va[b][i], w0, w1);
                 }
             }
