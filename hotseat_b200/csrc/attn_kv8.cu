@@ -3,8 +3,9 @@
 // Codes are integers of at most 127, which f16 holds exactly, so both
 // products run on the tensor cores with the codes as one operand and no loss:
 // the scales are taken outside, on the scores (K) and on the weights (V). The
-// other operand is an f16 pair hi + lo (22 bits) for f32 rows, one f16 for
-// 16-bit rows, after scaling by powers of two that keep it in f16's range:
+// other operand, f32 rows' q and every type's weights, is an f16 pair hi + lo
+// (22 bits; q of 16 bits is exact in one f16), after scaling by powers of two that
+// keep it in f16's range:
 //   q:       its largest element to [2^13, 2^14)
 //   weights: w = exp(S - m) s_v 2^(10 - e), 2^e at or above the largest s_v so
 //            far (of all that the CTA will meet, in chunks), so that weights down
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 // product of pairs counted once).
 template <int HD, int DT>
 struct ChunkGeom {
-    static constexpr bool QPAIR = DT == HS_F32, WPAIR = DT != HS_BF16;
+    static constexpr bool QPAIR = DT == HS_F32;
     static constexpr uint32_t KT = 128, ROWS = 256;
     // f32 rows take each tile's O' out of TMEM and sum it in registers, rounded
     // to nearest: left to grow there, 2,048 positions were 1.7e-6 off (the
@@ -608,17 +609,10 @@ struct ChunkGeom {
     static constexpr uint32_t NB = HD == 128 && QPAIR ? 1 : 2;  // K and V buffers
     static constexpr uint32_t Q_AT = 0, K_AT = Q_AT + 2 * (QPAIR ? 2 : 1) * Q_BYTES, V_AT = K_AT + NB * K_BYTES;
     static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: K [NB][128], V [NB][128]
-    static constexpr uint32_t BYTES = SC_AT + (DT == HS_BF16 ? 0 : NB * 2 * KT * 4) + 1024;
+    static constexpr uint32_t BYTES = SC_AT + NB * 2 * KT * 4 + 1024;
     static_assert(SC_AT >= ROWS * HD * 4, "the outputs fit where the operands were");
     static constexpr uint32_t S_COL = 0, O_COL = 256;       // TMEM columns: S of both tiles, O' of both
-    // bf16 rows take the scales with the codes (K and V rounded to f16, 2^-11 a
-    // value against the 2^-8 of their own type): 2.5 operations a score less.
-    // The others keep them outside, on scores and weights.
-    static constexpr bool FOLD = DT == HS_BF16;
-    // 2^VEXP is at least the largest V scale (FOLD: of the codes' f16 rows) and
-    // 2^PEXP what a weight of 1 is stored as
-    static constexpr uint32_t VEXP = FOLD ? 8 : 10;
-    static constexpr float PEXP = FOLD ? 8.0f : 0.0f;
+    static constexpr uint32_t VEXP = 10;                    // the largest V scale stands just under 2^VEXP
 };
 
 constexpr uint32_t kChunkLimit = 1u << 22;
@@ -667,7 +661,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t kfull[NB], kempty[NB], vfull[NB], vempty[NB], s_done[2], o_done[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ float ktop[16], vtop[16], row_cf[G::ROWS];
+    __shared__ float vtop[16], row_cf[G::ROWS];
     __shared__ uint64_t row_q[G::ROWS], row_out[G::ROWS];  // element offsets of the tile's rows
     __shared__ float row_m[SPLIT ? G::ROWS : 1], row_l[SPLIT ? G::ROWS : 1];
     // the warp's number as a value that is the same for its lanes
@@ -740,34 +734,28 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         tc5::alloc(&tmem_slot, 512);
         tc5::relinquish();
     }
-    // the largest scales that this CTA will meet, and powers of two to put them under
+    // the largest V scale that this CTA will meet, and a power of two to put it under
     const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
     const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, first >> a.kv.block_shift));
     const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, first >> a.kv.block_shift));
     {
-        float kt = 0.0f, vt = 0.0f;
-        for (uint32_t i = tid; i <= (end - 1) >> a.kv.block_shift; i += G::THREADS) {
-            if constexpr (G::FOLD) kt = fmaxf(kt, __ldg(ksp + i * a.kv.sblk_stride));
-            vt = fmaxf(vt, __ldg(vsp + i * a.kv.sblk_stride));
-        }
+        float vt = 0.0f;
+        for (uint32_t i = tid; i <= (end - 1) >> a.kv.block_shift; i += G::THREADS) vt = fmaxf(vt, __ldg(vsp + i * a.kv.sblk_stride));
 #pragma unroll
-        for (uint32_t d = 16; d > 0; d >>= 1) {
-            if constexpr (G::FOLD) kt = fmaxf(kt, __shfl_xor_sync(0xffffffffu, kt, d));
-            vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
-        }
-        if (lane == 0) ktop[warp] = kt, vtop[warp] = vt;
+        for (uint32_t d = 16; d > 0; d >>= 1) vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
+        if (lane == 0) vtop[warp] = vt;
     }
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
     const uint32_t tmem = tmem_slot;
-    // 2^exp over the power of two above the largest of them (1 if they are all 0), and its inverse
-    auto fit_under = [](const float* tops, uint32_t exp, float* inverse) {
+    // 2^VEXP over the power of two above it (1 if it is 0), and its inverse
+    auto fit_v = [&](float* inverse) {
         float top = 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < G::THREADS / 32; i++) top = fmaxf(top, tops[i]);
-        const uint32_t e = top > 0.0f ? min((__float_as_uint(top) >> 23) + 1, 253u) : 127u + exp;
-        const uint32_t bits = min(254u + exp - e, 253u);
+        for (uint32_t i = 0; i < G::THREADS / 32; i++) top = fmaxf(top, vtop[i]);
+        const uint32_t e = top > 0.0f ? min((__float_as_uint(top) >> 23) + 1, 253u) : 127u + G::VEXP;
+        const uint32_t bits = min(254u + G::VEXP - e, 253u);
         *inverse = __uint_as_float((254u - bits) << 23);
         return __uint_as_float(bits << 23);
     };
@@ -794,8 +782,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         constexpr uint32_t CPR = HD / 16, RPP = 32 / CPR, KP = 16 / RPP;
         const uint32_t kc = lane % CPR, kr = lane / CPR;
         float unit;
-        const float vfit = fit_under(vtop, G::VEXP, &unit);
-        const float kfit = G::FOLD ? fit_under(ktop, 7, &unit) : 1.0f;
+        const float vfit = fit_v(&unit);
         // V: four codes of each of eight positions (a 16-byte piece of a
         // transposed row), of position group vg, then vg + 1 where HD = 128.
         // Element d = 4 dw + e goes to row e * HD / 4 + dw, so that the lanes'
@@ -834,12 +821,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         auto load_s = [&](uint32_t t, uint32_t u) {  // the position of lane % 16; behind the end: 0
             const uint32_t p = t * KT + u * SP + 16 * cw + lane % 16;
             const float* at = ksp + (uint64_t)(min(p, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride;
-            ks[u] = p < end ? __ldg(at) * kfit : 0.0f;
+            ks[u] = p < end ? __ldg(at) : 0.0f;
             vs[u] = p < end ? __ldg(at + a.kv.splane / 4) * vfit : 0.0f;
-        };
-        auto times = [](uint32_t x, uint32_t h) {
-            const __half2 y = __hmul2(*reinterpret_cast<__half2*>(&x), *reinterpret_cast<__half2*>(&h));
-            return *reinterpret_cast<const uint32_t*>(&y);
         };
         // places in the tiles of buffer 0: of a chunk's first half (the second
         // lies beside it), of the pieces' row dw (the others DW rows on)
@@ -849,21 +832,10 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         for (uint32_t u = 0; u < G::SUB; u++) load_s(0, u), load_k(0, u), load_v(0, u);
         for (uint32_t t = 0; t < tiles; t++) {
             const uint32_t b = t % NB, use = t / NB;
-            uint32_t kh[G::SUB], vh[G::SUB];  // FOLD: position lane % 16's scale twice; positions 2 i, 2 i + 1 of lane i's
             float ks_now[G::SUB], vs_now[G::SUB];
 #pragma unroll
             for (uint32_t u = 0; u < G::SUB; u++) {
                 ks_now[u] = ks[u], vs_now[u] = vs[u];
-                if constexpr (G::FOLD) {
-                    // A NaN in either scale goes to the scores, where only the rows
-                    // that see the position take it; V's row is then zeros.
-                    const bool bad = isnan(vs[u]);
-                    const __half2 k2 = __float2half2_rn(bad ? vs[u] : ks[u]);
-                    kh[u] = *reinterpret_cast<const uint32_t*>(&k2);
-                    const uint32_t v1 = __half_as_ushort(__float2half_rn(bad ? 0.0f : vs[u]));
-                    const uint32_t v0 = __shfl_sync(0xffffffffu, v1, 2 * lane), v2 = __shfl_sync(0xffffffffu, v1, 2 * lane + 1);
-                    vh[u] = v0 | v2 << 16;
-                }
                 if (t + 1 < tiles) load_s(t + 1, u);
             }
             if (use > 0) wait(&kempty[b], (use - 1) & 1);
@@ -873,13 +845,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                 for (uint32_t i = 0; i < KP; i++) {
                     const uint4 w = kw[u][i];
                     // codes 0, 2, 1, 3 of every four, as q's elements lie
-                    uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
-                    uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
-                    if constexpr (G::FOLD) {
-                        const uint32_t h = __shfl_sync(0xffffffffu, kh[u], kr + i * RPP);
-                        x = make_uint4(times(x.x, h), times(x.y, h), times(x.z, h), times(x.w, h));
-                        y = make_uint4(times(y.x, h), times(y.y, h), times(y.z, h), times(y.w, h));
-                    }
+                    const uint4 x = make_uint4(even_bytes(w.x), odd_bytes(w.x), even_bytes(w.y), odd_bytes(w.y));
+                    const uint4 y = make_uint4(even_bytes(w.z), odd_bytes(w.z), even_bytes(w.w), odd_bytes(w.w));
                     // rows RPP apart: their places' swizzle is the same where RPP is 8, else it flips bit 2
                     const uint32_t row = b * G::K_BYTES + (u * SP + i * RPP) * 128, flip = RPP == 4 && (i & 1) ? 64 : 0;
                     sts128((to_k ^ flip) + row, x);
@@ -894,19 +861,12 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             if (use > 0) wait(&vempty[b], (use - 1) & 1);
 #pragma unroll
             for (uint32_t u = 0; u < G::SUB; u++) {
-                if constexpr (!G::FOLD) {
-                    if (lane < 16) {  // scales go with V: they are read until the weights are written
-                        sc[b * 2 * KT + u * SP + 16 * cw + lane] = ks_now[u];
-                        sc[b * 2 * KT + KT + u * SP + 16 * cw + lane] = vs_now[u];
-                    }
+                if (lane < 16) {  // scales go with V: they are read until the weights are written
+                    sc[b * 2 * KT + u * SP + 16 * cw + lane] = ks_now[u];
+                    sc[b * 2 * KT + KT + u * SP + 16 * cw + lane] = vs_now[u];
                 }
 #pragma unroll
                 for (uint32_t v = 0; v < VP; v++) {
-                    uint32_t h[4];
-                    if constexpr (G::FOLD) {
-#pragma unroll
-                        for (uint32_t p = 0; p < 4; p++) h[p] = __shfl_sync(0xffffffffu, vh[u], 4 * (VP == 2 ? v : lane / DW) + p);
-                    }
                     // elements d, d + 1, then d + 2, d + 3, by position pairs; group
                     // vg + 1's pieces lie beside group vg's: vg is even there
                     const uint32_t to = (to_v ^ (16 * v)) + b * G::V_BYTES + u * (SP / 64 * HD * 128);
@@ -917,7 +877,6 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                         for (uint32_t p = 0; p < 4; p++) {
                             const uint32_t x = __byte_perm(vw[u][v][2 * p], vw[u][v][2 * p + 1], e == 0 ? 0x5410 : 0x7632);
                             f[0][p] = even_bytes(x), f[1][p] = odd_bytes(x);
-                            if constexpr (G::FOLD) f[0][p] = times(f[0][p], h[p]), f[1][p] = times(f[1][p], h[p]);
                         }
                         sts128(to + e * (DW * 128), make_uint4(f[0][0], f[0][1], f[0][2], f[0][3]));
                         sts128(to + (e + 1) * (DW * 128), make_uint4(f[1][0], f[1][1], f[1][2], f[1][3]));
@@ -987,9 +946,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                 }
             }
             __syncwarp();
-            float kunit = 1.0f;
-            if constexpr (G::FOLD) fit_under(ktop, 7, &kunit);
-            const float cf = row_cf[row] * kunit;
+            const float cf = row_cf[row];
             fence_proxy_async_smem();
             bar_sync(1 + w);
 
@@ -1024,8 +981,8 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
 #pragma unroll
                     for (uint32_t k = 0; k < KT / 16; k++) {
                         const uint32_t at = k / 4 * (HD * 128 / 16) + 2 * (k % 4);
-                        if constexpr (G::WPAIR) tc5::mma_ts(ocol, scol + k * 16 + 8, vd + at, tc5::idesc_f16(128, HD), k > 0 || more);
-                        tc5::mma_ts(ocol, scol + k * 16, vd + at, tc5::idesc_f16(128, HD), G::WPAIR || k > 0 || more);
+                        tc5::mma_ts(ocol, scol + k * 16 + 8, vd + at, tc5::idesc_f16(128, HD), k > 0 || more);
+                        tc5::mma_ts(ocol, scol + k * 16, vd + at, tc5::idesc_f16(128, HD), true);
                     }
                     tc5::commit(&o_done[w]);
                     tc5::commit(&vempty[b]);
@@ -1036,15 +993,13 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             if (issuer) issue_s(0);
 
             float mx = -INFINITY, l = 0.0f;  // the running maximum in powers of two
-            // Columns 16 c.. of the scores, under K's scales where these are outside.
+            // Columns 16 c.. of the scores, under K's scales.
             auto scaled = [&](const float* ks, uint32_t c, float* x) {
-                if constexpr (!G::FOLD) {
 #pragma unroll
-                    for (uint32_t i = 0; i < 16; i += 4) {
-                        const float4 k4 = *reinterpret_cast<const float4*>(ks + 16 * c + i);
-                        mul2(x + i, k4.x, k4.y);
-                        mul2(x + i + 2, k4.z, k4.w);
-                    }
+                for (uint32_t i = 0; i < 16; i += 4) {
+                    const float4 k4 = *reinterpret_cast<const float4*>(ks + 16 * c + i);
+                    mul2(x + i, k4.x, k4.y);
+                    mul2(x + i + 2, k4.z, k4.w);
                 }
             };
             auto largest = [&](auto masked, uint32_t c, const float* x, float top, int left) {
@@ -1074,21 +1029,19 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                     }
                     add2(sum, x + i);
                     add2(sum, x + i + 2);
-                    if constexpr (!G::FOLD) {
-                        const float4 v4 = *reinterpret_cast<const float4*>(vs + 16 * c + i);
-                        mul2(x + i, v4.x, v4.y);
-                        mul2(x + i + 2, v4.z, v4.w);
-                        if constexpr (decltype(masked)::value) {  // a scale of NaN does not reach rows before it
+                    const float4 v4 = *reinterpret_cast<const float4*>(vs + 16 * c + i);
+                    mul2(x + i, v4.x, v4.y);
+                    mul2(x + i + 2, v4.z, v4.w);
+                    if constexpr (decltype(masked)::value) {  // a scale of NaN does not reach rows before it
 #pragma unroll
-                            for (uint32_t e = 0; e < 4; e++)
-                                if ((int)(16 * c + i + e) > left) x[i + e] = 0.0f;
-                        }
+                        for (uint32_t e = 0; e < 4; e++)
+                            if ((int)(16 * c + i + e) > left) x[i + e] = 0.0f;
                     }
                     pair16(x[i], x[i + 1], &wh[i / 2], &wl[i / 2]);
                     pair16(x[i + 2], x[i + 3], &wh[i / 2 + 1], &wl[i / 2 + 1]);
                 }
                 tc5::st8(scol + lanes + 16 * c, wh);
-                if constexpr (G::WPAIR) tc5::st8(scol + lanes + 16 * c + 8, wl);
+                tc5::st8(scol + lanes + 16 * c + 8, wl);
             };
             float o[G::OREG ? HD : 1], alpha = 1.0f;  // OREG: the outputs, and what they take when tile t's are added
 #pragma unroll
@@ -1147,7 +1100,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                         tc5::st16(ocol + lanes + 16 * c, reinterpret_cast<const uint32_t*>(y));
                     }
                 }
-                const float off = (mx == -INFINITY ? 0.0f : -mx) + G::PEXP;
+                const float off = mx == -INFINITY ? 0.0f : -mx;
                 float sum[2] = {0.0f, 0.0f};
 #pragma unroll 1
                 for (uint32_t c = 0; c < 8; c += 2) {
@@ -1194,7 +1147,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             // what a row's outputs are divided by goes through shared memory: the
             // registers of this loop stay its own (rows that see nothing: sums of 0)
             float vunit;
-            fit_under(vtop, G::VEXP, &vunit);
+            fit_v(&vunit);
             if constexpr (SPLIT) row_cf[row] = vunit, row_m[row] = mx, row_l[row] = l;
             else row_cf[row] = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
         }

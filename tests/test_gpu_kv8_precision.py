@@ -42,7 +42,7 @@ def run(form, s, q, n):
     return out.float().cpu().numpy()
 
 
-FORMS = ["single"]
+FORMS = ["single", "chunk"]
 
 
 @pytest.mark.parametrize("form", FORMS)
