@@ -7,9 +7,9 @@
 // (22 bits; q of 16 bits is exact in one f16), after scaling by powers of two that
 // keep it in f16's range:
 //   q:       its largest element to [2^13, 2^14)
-//   weights: w = exp(S - m) s_v 2^(10 - e), 2^e at or above the largest s_v so
-//            far (of all that the CTA will meet, in chunks), so that weights down
-//            to 2^-34 of the largest still count
+//   weights: w = exp(S - m) s_v 2^(10 - e), 2^e at or above the largest s_v that
+//            the row has seen so far, so that weights down to 2^-34 of the largest
+//            still count, and what a row does not see does not matter
 // Scores, statistics and sums are f32.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -608,11 +608,14 @@ struct ChunkGeom {
     static constexpr uint32_t K_BYTES = HD / 64 * SLAB, V_BYTES = 2 * HD * 128;
     static constexpr uint32_t NB = HD == 128 && QPAIR ? 1 : 2;  // K and V buffers
     static constexpr uint32_t Q_AT = 0, K_AT = Q_AT + 2 * (QPAIR ? 2 : 1) * Q_BYTES, V_AT = K_AT + NB * K_BYTES;
-    static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: K [NB][128], V [NB][128]
-    static constexpr uint32_t BYTES = SC_AT + NB * 2 * KT * 4 + 1024;
+    static constexpr uint32_t SC_AT = V_AT + NB * V_BYTES;  // scales: [NB][K 128 | V 128 | units 8]
+    static constexpr uint32_t SC = 2 * KT + KT / 16;        // floats of a buffer's scales, with V's unit for each 16
+    static constexpr uint32_t BYTES = SC_AT + NB * SC * 4 + 1024;
     static_assert(SC_AT >= ROWS * HD * 4, "the outputs fit where the operands were");
     static constexpr uint32_t S_COL = 0, O_COL = 256;       // TMEM columns: S of both tiles, O' of both
-    static constexpr uint32_t VEXP = 10;                    // the largest V scale stands just under 2^VEXP
+    // V's scales stand in shared memory in units of 2^e, e for 16 positions, the
+    // largest of them just under 2^VEXP
+    static constexpr int VEXP = 10, UNIT_MIN = -126;
 };
 
 constexpr uint32_t kChunkLimit = 1u << 22;
@@ -661,7 +664,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ uint64_t kfull[NB], kempty[NB], vfull[NB], vempty[NB], s_done[2], o_done[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ float vtop[16], row_cf[G::ROWS];
+    __shared__ float row_cf[G::ROWS];
     __shared__ uint64_t row_q[G::ROWS], row_out[G::ROWS];  // element offsets of the tile's rows
     __shared__ float row_m[SPLIT ? G::ROWS : 1], row_l[SPLIT ? G::ROWS : 1];
     // the warp's number as a value that is the same for its lanes
@@ -734,32 +737,12 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         tc5::alloc(&tmem_slot, 512);
         tc5::relinquish();
     }
-    // the largest V scale that this CTA will meet, and a power of two to put it under
     const uint8_t* base = reinterpret_cast<const uint8_t*>(a.kv.base[slot]);
-    const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, first >> a.kv.block_shift));
-    const float* vsp = reinterpret_cast<const float*>(base + a.kv.scale_off(1, kvh, first >> a.kv.block_shift));
-    {
-        float vt = 0.0f;
-        for (uint32_t i = tid; i <= (end - 1) >> a.kv.block_shift; i += G::THREADS) vt = fmaxf(vt, __ldg(vsp + i * a.kv.sblk_stride));
-#pragma unroll
-        for (uint32_t d = 16; d > 0; d >>= 1) vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
-        if (lane == 0) vtop[warp] = vt;
-    }
     tc5::fence_before();
     __syncthreads();
     tc5::fence_after();
     const uint32_t tmem = tmem_slot;
-    // 2^VEXP over the power of two above it (1 if it is 0), and its inverse
-    auto fit_v = [&](float* inverse) {
-        float top = 0.0f;
-#pragma unroll
-        for (uint32_t i = 0; i < G::THREADS / 32; i++) top = fmaxf(top, vtop[i]);
-        const uint32_t e = top > 0.0f ? min((__float_as_uint(top) >> 23) + 1, 253u) : 127u + G::VEXP;
-        const uint32_t bits = min(254u + G::VEXP - e, 253u);
-        *inverse = __uint_as_float((254u - bits) << 23);
-        return __uint_as_float(bits << 23);
-    };
-    float* sc = reinterpret_cast<float*>(smem + G::SC_AT);  // [NB][K 128 | V 128]
+    float* sc = reinterpret_cast<float*>(smem + G::SC_AT);  // [NB][G::SC]
     // A wait that runs out marks the call and no longer waits: every thread
     // still passes every barrier, and the CTA ends.
     bool dead = false;
@@ -781,8 +764,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
         // K: a lane takes 16 codes of rows kr, kr + RPP, ...
         constexpr uint32_t CPR = HD / 16, RPP = 32 / CPR, KP = 16 / RPP;
         const uint32_t kc = lane % CPR, kr = lane / CPR;
-        float unit;
-        const float vfit = fit_v(&unit);
+        const float* ksp = reinterpret_cast<const float*>(base + a.kv.scale_off(0, kvh, first >> a.kv.block_shift));
         // V: four codes of each of eight positions (a 16-byte piece of a
         // transposed row), of position group vg, then vg + 1 where HD = 128.
         // Element d = 4 dw + e goes to row e * HD / 4 + dw, so that the lanes'
@@ -822,7 +804,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             const uint32_t p = t * KT + u * SP + 16 * cw + lane % 16;
             const float* at = ksp + (uint64_t)(min(p, end - 1) >> a.kv.block_shift) * a.kv.sblk_stride;
             ks[u] = p < end ? __ldg(at) : 0.0f;
-            vs[u] = p < end ? __ldg(at + a.kv.splane / 4) * vfit : 0.0f;
+            vs[u] = p < end ? __ldg(at + a.kv.splane / 4) : 0.0f;
         };
         // places in the tiles of buffer 0: of a chunk's first half (the second
         // lies beside it), of the pieces' row dw (the others DW rows on)
@@ -861,10 +843,14 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             if (use > 0) wait(&vempty[b], (use - 1) & 1);
 #pragma unroll
             for (uint32_t u = 0; u < G::SUB; u++) {
-                if (lane < 16) {  // scales go with V: they are read until the weights are written
-                    sc[b * 2 * KT + u * SP + 16 * cw + lane] = ks_now[u];
-                    sc[b * 2 * KT + KT + u * SP + 16 * cw + lane] = vs_now[u];
-                }
+                // scales go with V: they are read until the weights are written
+                float top = fmaxf(vs_now[u], 0.0f);  // (a NaN is skipped)
+#pragma unroll
+                for (uint32_t d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const int unit = max((int)(__float_as_uint(top) >> 23) - 126 - G::VEXP, G::UNIT_MIN);  // at most 128 - VEXP + 1
+                float* to_s = sc + b * G::SC + u * SP + 16 * cw;
+                if (lane < 16) to_s[lane] = ks_now[u], to_s[KT + lane] = vs_now[u] * __uint_as_float((127u - unit) << 23);
+                if (lane == 0) sc[b * G::SC + 2 * KT + u * (SP / 16) + cw] = (float)unit;
 #pragma unroll
                 for (uint32_t v = 0; v < VP; v++) {
                     // elements d, d + 1, then d + 2, d + 3, by position pairs; group
@@ -992,7 +978,12 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             const bool issuer = warp % 4 == 0;
             if (issuer) issue_s(0);
 
-            float mx = -INFINITY, l = 0.0f;  // the running maximum in powers of two
+            // The running maximum in powers of two (a whole number, so that it and the
+            // units add up exactly), the sum of weights, the unit of the outputs.
+            float mx = -INFINITY, l = 0.0f, un = G::UNIT_MIN;
+            auto pow2f = [](float e) {  // a whole number -127 (gives 0) .. 127
+                return __uint_as_float((__float_as_uint(12582912.0f + e) + 127u) << 23);
+            };
             // Columns 16 c.. of the scores, under K's scales.
             auto scaled = [&](const float* ks, uint32_t c, float* x) {
 #pragma unroll
@@ -1013,10 +1004,39 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                 }
                 return top;
             };
+            // The largest unit that this row sees of a tile; of a group of 16 that it sees
+            // in part, by the scales that it does see.
+            auto largest_unit = [&](auto masked, const float* vs, int left) {
+                const float* us = vs + KT;
+                float u = G::UNIT_MIN;
+                if constexpr (decltype(masked)::value) {
+                    const int whole = (left + 1) >> 4, part = (left + 1) & 15;
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        if (c < whole) u = fmaxf(u, us[c]);
+                    if (left >= 0 && left < (int)KT - 1 && part) {
+                        float top = 0.0f;
+#pragma unroll 1
+                        for (int i = 0; i < part; i++) top = fmaxf(top, vs[16 * whole + i]);
+                        if (top > 0.0f) u = fmaxf(u, us[whole] + (float)((int)(__float_as_uint(top) >> 23) - 126 - G::VEXP));
+                    }
+                } else {
+                    const float4 a4 = *reinterpret_cast<const float4*>(us), b4 = *reinterpret_cast<const float4*>(us + 4);
+                    u = fmaxf(fmaxf(fmaxf(a4.x, a4.y), fmaxf(a4.z, a4.w)), fmaxf(fmaxf(b4.x, b4.y), fmaxf(b4.z, b4.w)));
+                }
+                return u;
+            };
             // Weights of columns 16 c.. into TMEM over their scores (hi in the first
-            // eight columns, lo in the others); adds their sum.
-            auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left, float* sum) {
+            // eight columns, lo in the others); adds their sum. A weight is formed times
+            // 2^d, d its group's unit over the outputs' (0 or less where the group is seen
+            // whole), and summed without it. Far below, where the group adds nothing,
+            // d is cut; so it is far above, where a group's other values, 2^100 times
+            // larger, are hidden.
+            auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left, float* total) {
                 uint32_t wh[8], wl[8];
+                float d = fmaxf(vs[KT + c] - un, -60.0f), sum[2] = {0.0f, 0.0f};
+                if constexpr (decltype(masked)::value) d = fminf(d, 100.0f);
+                off += d;
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i += 4) {
                     fma2(x + i, cf, off);
@@ -1040,6 +1060,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                     pair16(x[i], x[i + 1], &wh[i / 2], &wl[i / 2]);
                     pair16(x[i + 2], x[i + 3], &wh[i / 2 + 1], &wl[i / 2 + 1]);
                 }
+                *total = fmaf(sum[0] + sum[1], pow2f(-d), *total);
                 tc5::st8(scol + lanes + 16 * c, wh);
                 tc5::st8(scol + lanes + 16 * c + 8, wl);
             };
@@ -1062,7 +1083,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             // weights, so that few registers hold them; the next columns are on
             // their way from TMEM while these are worked on.
             auto tile = [&](auto masked, uint32_t t, int left) {
-                const float *ks = sc + t % NB * 2 * KT, *vs = ks + KT;
+                const float *ks = sc + t % NB * G::SC, *vs = ks + KT;
                 float top = -INFINITY, x[16], y[16];
                 tc5::ld16(scol + lanes, x);
 #pragma unroll 1
@@ -1083,10 +1104,19 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                     }
                 }
                 top *= cf;
-                const bool up = top > mx + kSlack;
-                alpha = up ? ex2(mx - top) : 1.0f;
-                l *= alpha;
-                mx = up ? top : mx;
+                const float u = fmaxf(un, largest_unit(masked, vs, left));
+                const bool up = top > mx + kSlack || u > un;
+                if (top > mx + kSlack) {
+                    top = ceilf(top);
+                    alpha = ex2(mx - top);
+                    l *= alpha;
+                    mx = top;
+                } else {
+                    alpha = 1.0f;
+                }
+                alpha *= pow2f(fmaxf(un - u, -127.0f));
+                un = u;
+                __syncwarp();
                 if (!G::OREG && t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum
                     tc5::wait_ld();
                     wait(&o_done[w], (t - 1) & 1);
@@ -1101,19 +1131,19 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                     }
                 }
                 const float off = mx == -INFINITY ? 0.0f : -mx;
-                float sum[2] = {0.0f, 0.0f};
+                float sum = 0.0f;
 #pragma unroll 1
                 for (uint32_t c = 0; c < 8; c += 2) {
                     tc5::wait_ld();
                     tc5::ld16(scol + lanes + 16 * (c + 1), y);
                     scaled(ks, c, x);
-                    weights(masked, vs, c, x, off, left, sum);
+                    weights(masked, vs, c, x, off, left, &sum);
                     tc5::wait_ld();
                     if (c < 6) tc5::ld16(scol + lanes + 16 * (c + 2), x);
                     scaled(ks, c + 1, y);
-                    weights(masked, vs, c + 1, y, off, left, sum);
+                    weights(masked, vs, c + 1, y, off, left, &sum);
                 }
-                l += sum[0] + sum[1];
+                l += sum;
             };
             for (uint32_t t = 0; t < tiles; t++) {
                 const int left = lim - (int)(t * KT);  // columns 0..left are seen
@@ -1146,8 +1176,7 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             }
             // what a row's outputs are divided by goes through shared memory: the
             // registers of this loop stay its own (rows that see nothing: sums of 0)
-            float vunit;
-            fit_v(&vunit);
+            const float vunit = pow2f(un);
             if constexpr (SPLIT) row_cf[row] = vunit, row_m[row] = mx, row_l[row] = l;
             else row_cf[row] = lim >= 0 ? vunit * __frcp_rn(l) : 0.0f;
         }

@@ -83,3 +83,27 @@ def test_large_scores_near_one_another(form, dtype, hd, nh, nkv, block):
     got, qf = run(form, s, q, n), q.float().cpu().numpy()
     for r in range(n):
         close(got[r], *ref.attend(qf[r], r, hd ** -0.5), hd, r + 1, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("times", [2.0 ** 12, 2.0 ** 40, 2.0 ** 90])
+@pytest.mark.parametrize("hd, nh, nkv, block, n, lo, rise", [
+    (64, 7, 1, 1, 300, 100, 200), (128, 12, 2, 16, 300, 100, 160), (64, 4, 2, 1, 290, 0, 1), (64, 3, 1, 1, 4400, 4110, 4300),
+    (128, 2, 2, 32, 4300, 4100, 4128)])
+def test_large_values_behind_a_row_do_not_reach_it(dtype, times, hd, nh, nkv, block, n, lo, rise):
+    """K and V from position `rise` on are far larger than before it: rows before it keep their precision."""
+    rng = np.random.default_rng(n + hd)
+    kv, ref = hs.Kv.alloc8(hs.KvSpec(1, nkv, hd, n, 0), block=block), Cache(nkv, hd, n, block)
+    s = hs.Kv8Set([kv], n_heads=nh)
+    k, v = (rng.standard_normal((n, nkv, hd)).astype(np.float32) for _ in range(2))
+    k[rise:] *= np.float32(times)
+    v[rise:] *= np.float32(times)
+    s.append(0, dev(k), dev(v), i32([0]), i32([0, n]))
+    ref.append(0, k, v)
+    q = dev((rng.standard_normal((n - lo, nh, hd)) * 0.3).astype(np.float32), DT[dtype])
+    out = torch.empty_like(q)
+    s.attend(0, q, out, i32([lo]), i32([0, n - lo]))
+    s.check()
+    got, qf = out.float().cpu().numpy(), q.float().cpu().numpy()
+    for p in sorted({lo, rise - 1, (lo + rise) // 2, max(lo, rise - 7)}):
+        close(got[p - lo], *ref.attend(qf[p - lo], p, hd ** -0.5), hd, p + 1, dtype)
