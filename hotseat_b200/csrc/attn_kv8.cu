@@ -635,9 +635,9 @@ __device__ __forceinline__ void fma2(float* x, float a, float b) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(a, a)), "l"(pack2(b, b)));
     unpack2(r, x, x + 1);
 }
-__device__ __forceinline__ void add2(float* x, const float* y) {
+__device__ __forceinline__ void add2(float* x, float a, float b) {
     uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(y[0], y[1])));
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x[0], x[1])), "l"(pack2(a, b)));
     unpack2(r, x, x + 1);
 }
 
@@ -1031,24 +1031,32 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             // 2^d, d its group's unit over the outputs' (0 or less where the group is seen
             // whole), and summed without it. Far below, where the group adds nothing,
             // d is cut; so it is far above, where a group's other values, 2^100 times
-            // larger, are hidden.
+            // larger, are hidden. The masked form also takes scores whose product with cf
+            // has to be rounded as their maximum was, lest the two part by whole powers of two.
             auto weights = [&](auto masked, const float* vs, uint32_t c, float* x, float off, int left, float* total) {
                 uint32_t wh[8], wl[8];
                 float d = fmaxf(vs[KT + c] - un, -60.0f), sum[2] = {0.0f, 0.0f};
                 if constexpr (decltype(masked)::value) d = fminf(d, 100.0f);
-                off += d;
+                else off += d;
 #pragma unroll
                 for (uint32_t i = 0; i < 16; i += 4) {
-                    fma2(x + i, cf, off);
-                    fma2(x + i + 2, cf, off);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e += 2) {
+                        if constexpr (decltype(masked)::value) {  // (as pairs, product and sum came out as one FMA)
+                            x[i + e] = __fadd_rn(__fadd_rn(__fmul_rn(x[i + e], cf), off), d);
+                            x[i + e + 1] = __fadd_rn(__fadd_rn(__fmul_rn(x[i + e + 1], cf), off), d);
+                        } else {
+                            fma2(x + i + e, cf, off);
+                        }
+                    }
 #pragma unroll
                     for (uint32_t e = 0; e < 4; e++) {
                         x[i + e] = ex2(x[i + e]);
                         if constexpr (decltype(masked)::value)
                             if ((int)(16 * c + i + e) > left) x[i + e] = 0.0f;
                     }
-                    add2(sum, x + i);
-                    add2(sum, x + i + 2);
+                    add2(sum, x[i], x[i + 1]);
+                    add2(sum, x[i + 2], x[i + 3]);
                     const float4 v4 = *reinterpret_cast<const float4*>(vs + 16 * c + i);
                     mul2(x + i, v4.x, v4.y);
                     mul2(x + i + 2, v4.z, v4.w);
@@ -1082,9 +1090,9 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
             // One tile: the scores are read twice, for their maximum and for the
             // weights, so that few registers hold them; the next columns are on
             // their way from TMEM while these are worked on.
-            auto tile = [&](auto masked, uint32_t t, int left) {
-                const float *ks = sc + t % NB * G::SC, *vs = ks + KT;
-                float top = -INFINITY, x[16], y[16];
+            float x[16], y[16];
+            auto find_top = [&](auto masked, const float* ks, int left) {
+                float top = -INFINITY;
                 tc5::ld16(scol + lanes, x);
 #pragma unroll 1
                 for (uint32_t c = 0; c < 8; c += 2) {
@@ -1093,44 +1101,14 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                     scaled(ks, c, x);
                     top = largest(masked, c, x, top, left);
                     tc5::wait_ld();
-                    tc5::ld16(scol + lanes + 16 * ((c + 2) % 8), x);  // at last the first again
+                    if (c < 6) tc5::ld16(scol + lanes + 16 * (c + 2), x);
                     scaled(ks, c + 1, y);
                     top = largest(masked, c + 1, y, top, left);
                 }
-                if constexpr (G::OREG) {
-                    if (t > 0) {
-                        tc5::wait_ld();
-                        add_o(t - 1);
-                    }
-                }
-                top *= cf;
-                const float u = fmaxf(un, largest_unit(masked, vs, left));
-                const bool up = top > mx + kSlack || u > un;
-                if (top > mx + kSlack) {
-                    top = ceilf(top);
-                    alpha = ex2(mx - top);
-                    l *= alpha;
-                    mx = top;
-                } else {
-                    alpha = 1.0f;
-                }
-                alpha *= pow2f(fmaxf(un - u, -127.0f));
-                un = u;
-                __syncwarp();
-                if (!G::OREG && t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum
-                    tc5::wait_ld();
-                    wait(&o_done[w], (t - 1) & 1);
-                    tc5::fence_after();
-#pragma unroll 1
-                    for (uint32_t c = 0; c < HD / 16; c++) {
-                        tc5::ld16(ocol + lanes + 16 * c, y);
-                        tc5::wait_ld();
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; i++) y[i] *= alpha;
-                        tc5::st16(ocol + lanes + 16 * c, reinterpret_cast<const uint32_t*>(y));
-                    }
-                }
-                const float off = mx == -INFINITY ? 0.0f : -mx;
+                return top;
+            };
+            auto all_weights = [&](auto masked, const float* ks, float off, int left) {
+                const float* vs = ks + KT;
                 float sum = 0.0f;
 #pragma unroll 1
                 for (uint32_t c = 0; c < 8; c += 2) {
@@ -1150,8 +1128,46 @@ __global__ void __launch_bounds__(ChunkGeom<HD, DT>::THREADS, 1) k_kv8_chunk(con
                 wait(&vfull[t % NB], t / NB & 1);
                 wait(&s_done[w], t & 1);
                 tc5::fence_after();
-                if (__all_sync(0xffffffffu, left >= (int)KT - 1)) tile(std::false_type{}, t, left);
-                else tile(std::true_type{}, t, left);
+                const float* ks = sc + t % NB * G::SC;
+                const bool full = __all_sync(0xffffffffu, left >= (int)KT - 1);
+                float top, u;
+                if (full) top = find_top(std::false_type{}, ks, left), u = largest_unit(std::false_type{}, ks + KT, left);
+                else top = find_top(std::true_type{}, ks, left), u = largest_unit(std::true_type{}, ks + KT, left);
+                __syncwarp();
+                if constexpr (G::OREG) {
+                    if (t > 0) add_o(t - 1);
+                }
+                top *= cf;
+                u = fmaxf(un, u);
+                const bool up = top > mx + kSlack || u > un;
+                if (top > mx + kSlack) {
+                    top = ceilf(top);
+                    alpha = ex2(mx - top);
+                    l *= alpha;
+                    mx = top;
+                } else {
+                    alpha = 1.0f;
+                }
+                alpha *= pow2f(fmaxf(un - u, -127.0f));
+                un = u;
+                if (!G::OREG && t > 0 && __any_sync(0xffffffffu, up)) {  // outputs so far to the new maximum and unit
+                    wait(&o_done[w], (t - 1) & 1);
+                    tc5::fence_after();
+#pragma unroll 1
+                    for (uint32_t c = 0; c < HD / 16; c++) {
+                        tc5::ld16(ocol + lanes + 16 * c, y);
+                        tc5::wait_ld();
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; i++) y[i] *= alpha;
+                        tc5::st16(ocol + lanes + 16 * c, reinterpret_cast<const uint32_t*>(y));
+                    }
+                }
+                const float off = mx == -INFINITY ? 0.0f : -mx;
+                // a product with cf is off by less than a step of 2^-4 up to here
+                const bool small = __all_sync(0xffffffffu, fabsf(off) <= 1048576.0f);
+                tc5::ld16(scol + lanes, x);
+                if (full && small) all_weights(std::false_type{}, ks, off, left);
+                else all_weights(std::true_type{}, ks, off, left);
                 tc5::wait_st();
                 tc5::fence_before();
                 bar_sync(1 + w);

@@ -107,3 +107,43 @@ def test_large_values_behind_a_row_do_not_reach_it(dtype, times, hd, nh, nkv, bl
     got, qf = out.float().cpu().numpy(), q.float().cpu().numpy()
     for p in sorted({lo, rise - 1, (lo + rise) // 2, max(lo, rise - 7)}):
         close(got[p - lo], *ref.attend(qf[p - lo], p, hd ** -0.5), hd, p + 1, dtype)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [2.0 ** 22, 2.0 ** 26, 2.0 ** 45, 2.0 ** 100])
+@pytest.mark.parametrize("hd, nh, nkv", [(64, 7, 1), (128, 4, 2)])
+def test_scores_of_any_size(form, dtype, size, hd, nh, nkv):
+    """Scores of about `size`, the largest by a third: it takes all the weight. And rows whose scores are all alike."""
+    rng = np.random.default_rng(hd + 2)
+    n, m = 200, 60
+    kv, ref = hs.Kv.alloc8(hs.KvSpec(1, nkv, hd, n, 0)), Cache(nkv, hd, n, 1)
+    s = hs.Kv8Set([kv], n_heads=nh)
+    way = np.where(rng.random((1, nkv, hd)) < 0.5, -1.0, 1.0)
+    k = way * rng.uniform(0.25, 0.6, (n, nkv, 1))
+    k[100] = way[0]
+    v = rng.standard_normal((n, nkv, hd)).astype(np.float32)
+    k = k.astype(np.float32)
+    s.append(0, dev(k), dev(v), i32([0]), i32([0, n]))
+    ref.append(0, k, v)
+    # odd factors, so that no product of them is exact
+    q = np.repeat(way, nh // nkv, axis=1) * rng.uniform(1.1, 1.9, (m, nh, 1))
+    q = dev(q.astype(np.float32), DT[dtype])
+    scale = float(np.float32(size * 1.2345 / hd))
+    out = torch.full_like(q, 9.0)
+    one = lambda o: s.attend(0, q, o, i32([n - m]), i32([0, m]), scale=scale)  # noqa: E731
+    if form == "single":
+        one = lambda o: [s.attend(0, q[r:r + 1], o[r:r + 1], i32([n - m + r]), scale=scale) for r in range(m)]  # noqa: E731
+    one(out)
+    got = out.float().cpu().numpy()
+    top = ref.values(1, 100, 101)[0].astype(np.float64)[np.arange(nh) // (nh // nkv)]
+    err = np.abs(got - top) - np.abs(top) * torch.finfo(DT[dtype]).eps / 2
+    assert np.all(err <= 64 * U * np.abs(top).max()), np.max(err)
+    k[:] = k[:1]
+    s.append(0, dev(k), dev(v), i32([0]), i32([0, n]))
+    one(out)
+    got = out.float().cpu().numpy()
+    vals = ref.values(1, 0, n).astype(np.float64)
+    for r in (0, m - 1):
+        want = vals[:n - m + r + 1].mean(0)[np.arange(nh) // (nh // nkv)]
+        assert np.all(np.abs(got[r] - want) <= bound(want, 0, np.abs(vals).max(), hd, n, dtype))
