@@ -1991,8 +1991,10 @@ struct hs_batch {
     float* att_part = nullptr;     // split-KV attention partials [cap_slots][nkv][max_splits][record]
     uint32_t* att_cnt = nullptr;   // [cap_slots][nkv]
     // 8-bit regions (block8: their scale block, 0 for f32 ones), at their first
-    // use: rows of q, k, v and of the attention, positions, its workspace
+    // use: rows of q, k, v and of the attention, positions; at the first decode
+    // step over them, which joins8 tells, the workspace of single rows
     uint32_t block8 = 0;
+    bool joins8 = false;
     float *q8 = nullptr, *k8 = nullptr, *v8 = nullptr, *o8 = nullptr, *part8 = nullptr;
     uint32_t *pos8 = nullptr, *start8 = nullptr, *counters8 = nullptr;
     hs::Kv8Plan plan8;
@@ -2069,27 +2071,34 @@ int batch_gemm(hs_batch* b, const TcGemmPlan& p, const uint16_t* a_hi, const uin
     return HS_OK;
 }
 
-// Buffers and limits of 8-bit regions' attention, before any capture.
-int batch_ensure_kv8(hs_batch* b) {
-    if (b->q8) return HS_OK;
+// Buffers and limits of 8-bit regions' attention, before any capture. What a
+// call that failed had allocated stays for the next one.
+int batch_ensure_kv8(hs_batch* b, bool prefill) {
+    if (b->q8 && (prefill || b->joins8)) return HS_OK;
     const hs_config& c = b->m->cfg;
     const uint64_t C = b->cap_slots;
-    HS_CUDA_TRY(kv8_attend_set_smem_limits());
-    b->plan8 = kv8_plan(model_kv_spec(b->m, 0), c.n_heads, b->cap_slots);
     auto alloc = [&](auto** p, uint64_t count) -> int {
+        if (*p) return HS_OK;
         cudaError_t e = cudaMalloc(reinterpret_cast<void**>(p), std::max<uint64_t>(count, 1) * 4);
-        if (e != cudaSuccess) return fail(HS_E_NOMEM, std::string("cudaMalloc: ") + cudaGetErrorString(e));
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(HS_E_NOMEM, std::string("cudaMalloc: ") + cudaGetErrorString(e));
+        }
         return HS_OK;
     };
-    float* q8 = nullptr;  // set last: the sign that all are there
     int rc;
-    if ((rc = alloc(&b->k8, C * c.n_kv_heads * c.head_dim)) || (rc = alloc(&b->v8, C * c.n_kv_heads * c.head_dim)) ||
-        (rc = alloc(&b->o8, C * c.n_heads * c.head_dim)) || (rc = alloc(&b->pos8, C)) || (rc = alloc(&b->start8, 2)) ||
-        (rc = alloc(&b->part8, b->plan8.part_floats)) || (rc = alloc(&b->counters8, b->plan8.counters)) ||
-        (rc = alloc(&q8, C * c.n_heads * c.head_dim)))
-        return rc;
-    b->q8 = q8;
+    if (!b->q8) {
+        HS_CUDA_TRY(kv8_attend_set_smem_limits());
+        b->plan8 = kv8_plan(model_kv_spec(b->m, 0), c.n_heads, b->cap_slots);
+        if ((rc = alloc(&b->k8, C * c.n_kv_heads * c.head_dim)) || (rc = alloc(&b->v8, C * c.n_kv_heads * c.head_dim)) ||
+            (rc = alloc(&b->o8, C * c.n_heads * c.head_dim)) || (rc = alloc(&b->pos8, C)) ||
+            (rc = alloc(&b->start8, 2)) || (rc = alloc(&b->q8, C * c.n_heads * c.head_dim)))
+            return rc;
+    }
+    if (prefill) return HS_OK;  // chunks need no workspace
+    if ((rc = alloc(&b->part8, b->plan8.part_floats)) || (rc = alloc(&b->counters8, b->plan8.counters))) return rc;
     HS_CUDA_TRY(cudaMemsetAsync(b->counters8, 0, std::max<uint64_t>(b->plan8.counters, 1) * 4, b->st));
+    b->joins8 = true;
     return HS_OK;
 }
 
@@ -2316,7 +2325,7 @@ int batch_kv_tables(hs_batch* b, hs_kv* const* kvs, uint32_t n, bool same_sequen
             if (kvs[j] == kvs[i]) return fail(HS_E_ARG, "a KV region appears twice in one batch");
     }
     if (kvs[0]->block8) {
-        int rc = batch_ensure_kv8(b);
+        int rc = batch_ensure_kv8(b, same_sequence);
         if (rc) return rc;
     }
     b->block8 = kvs[0]->block8;
@@ -2467,7 +2476,7 @@ int hs_prefill(const hs_model* m, hs_kv* kv, const uint32_t* tokens, uint32_t n,
         if (tokens[i] >= m->cfg.vocab) return fail(HS_E_ARG, "token " + std::to_string(tokens[i]) + " out of range");
     HS_CUDA_TRY(cudaSetDevice(m->device));
     const uint32_t C = b->cap_slots;
-    if (m->pf_qblock && !b->pf_part)
+    if (m->pf_qblock && !kv->block8 && !b->pf_part)
         HS_CUDA_TRY(cudaMalloc(&b->pf_part, (size_t)C * m->cfg.n_kv_heads * m->pf_nseg *
                                                 attn_record(m->cfg.n_heads / m->cfg.n_kv_heads, m->cfg.head_dim) * 4));
     std::vector<hs_kv*> same(std::min(C, std::max(n, 1u)), kv);
