@@ -28,7 +28,7 @@ inline Kv8Geo kv8_geo(const hs_kv_spec& s, uint32_t block) {
     Kv8Geo g;
     g.layers = s.n_layers;
     g.plane = pad((uint64_t)s.max_ctx * s.n_kv_heads * s.head_dim);
-    g.splane = pad((uint64_t)((s.max_ctx + block - 1) / block) * s.n_kv_heads * 4);
+    g.splane = pad(((uint64_t)s.max_ctx + block - 1) / block * s.n_kv_heads * 4);
     return g;
 }
 // A shape that the 8-bit kernels take: HS_OK or an error.

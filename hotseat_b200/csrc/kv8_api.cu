@@ -21,8 +21,10 @@ int kv8_check_shape(const hs_kv_spec& s, uint32_t block) {
     if (s.head_dim != 64 && s.head_dim != 128) return fail(HS_E_UNSUPPORTED, "head_dim must be 64 or 128");
     if (block != 1 && block != 16 && block != 32 && block != 64 && block != 128)
         return fail(HS_E_UNSUPPORTED, "the scale block must be 1, 16, 32, 64 or 128 positions");
-    // offsets are 64 bits wide; the region itself must be addressable
-    if (s.n_kv_heads > 4096 || s.max_ctx > (1u << 30)) return fail(HS_E_UNSUPPORTED, "KV shape too large");
+    // offsets are 64 bits wide; the region itself must be addressable (a layer of
+    // the largest shape has 2^51 bytes, so the sum of layers could pass 64 bits)
+    if (s.n_kv_heads > 4096 || s.max_ctx > (1u << 30) || s.n_layers > (1ull << 48) / kv8_geo(s, block).layer_bytes())
+        return fail(HS_E_UNSUPPORTED, "KV shape too large");
     return HS_OK;
 }
 
@@ -122,7 +124,7 @@ uint64_t hs_kv8_live_ranges_between(const hs_kv_spec* s, uint32_t block, uint32_
     if (!s || !block || (block & (block - 1)) || to <= from) return 0;
     const Kv8Geo g = kv8_geo(*s, block);
     const uint64_t b0 = from / block, b1 = ((uint64_t)to + block - 1) / block, p0 = b0 * block;
-    const uint64_t nb = (s->max_ctx + block - 1) / block;
+    const uint64_t nb = ((uint64_t)s->max_ctx + block - 1) / block;
     uint64_t count = 0;
     // a plane's units [a, b): `w` bytes for each unit and head, n units a head
     auto plane = [&](uint64_t off, uint64_t a, uint64_t b, uint64_t w, uint64_t n) {

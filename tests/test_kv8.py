@@ -110,3 +110,19 @@ def test_values_stay_within_a_step_however_a_block_fills(block):
     whole.append(0, x, x)
     steps = whole.scales[0][np.arange(100) // block]
     assert np.all(np.abs(whole.values(0, 0, 100).astype(np.float64) - x) <= steps[:, :, None] * (0.5 + 2 ** -16))
+
+
+@pytest.mark.parametrize("spec, block", [((1 << 20, 4096, 128, 1 << 30, 0), 1), ((1 << 31, 4096, 128, 1 << 30, 1), 16),
+                                         ((0xFFFFFFFF, 1, 64, 1 << 30, 0), 128)])
+def test_regions_whose_bytes_pass_64_bits_are_refused(spec, block):
+    """2^20 layers of 2^50 + 2^45 bytes are 0 modulo 2^64: a region of no bytes, with layers behind it."""
+    with pytest.raises(hs.HotseatError) as e:
+        hs.Kv.alloc8(hs.KvSpec(*spec), block=block)
+    assert e.value.code == hs.HS_E_UNSUPPORTED
+
+
+def test_live_ranges_of_the_longest_context():
+    s = hs.KvSpec(1, 2, 64, 0xFFFFFFFF, 1)
+    got = hs.live_ranges_between8(s, 128, 0, 1)
+    plane = -(-0xFFFFFFFF * 2 * 64 // 256) * 256
+    assert got[4:6] == [(2 * plane, 4), (2 * plane + 4 * (1 << 25), 4)]  # the second head's scales behind the first's
