@@ -232,8 +232,9 @@ def lib():
 class Model:
     """A loaded model on one GPU (Model::load, model.rs:110-215)."""
 
-    def __init__(self, handle):
+    def __init__(self, handle, device=0):
         self._h = handle
+        self.device = device
         self.cfg = Config()
         _check(_lib.hs_model_config(handle, C.byref(self.cfg)))
 
@@ -243,7 +244,7 @@ class Model:
         NUMERIC_FAST (GPU-native reduction order, deterministic across GPUs)."""
         h = C.c_void_p()
         _check(_lib.hs_model_load_ex(os.fsencode(path), max_ctx, device, numeric, C.byref(h)))
-        return cls(h)
+        return cls(h, device)
 
     @property
     def fingerprint(self):
@@ -308,9 +309,10 @@ class Model:
 class Kv:
     """Device KV region in the reference's byte layout, with a dirty-page bitmap."""
 
-    def __init__(self, handle, model):
+    def __init__(self, handle, model, device=None):
         self._h = handle
         self.model = model
+        self.device = model.device if device is None else device
         self.spec = KvSpec()
         b, ps, npg = C.c_uint64(), C.c_uint32(), C.c_uint64()
         _check(_lib.hs_kv_info(handle, C.byref(self.spec), C.byref(b), C.byref(ps), C.byref(npg)))
@@ -332,7 +334,7 @@ class Kv:
         `block` positions and KV head, K and V apart (hs_kv8_alloc)."""
         h = C.c_void_p()
         _check(_lib.hs_kv8_alloc(device, C.byref(spec), block, page_size, fingerprint, C.byref(h)))
-        return cls(h, None)
+        return cls(h, None, device)
 
     def ipc_handle(self):
         """The region's CUDA IPC handle (bytes) for another process's open_ipc."""
@@ -531,7 +533,7 @@ class Kv8Set:
     """8-bit KV regions as the slots of batched calls (hs_kv8_set). Row
     matrices are device tensors [rows, heads, head_dim] (f32, f16 or bf16, any
     row and head strides); pos [n] and row_start [n + 1] are int32 device
-    tensors: slot i's rows are row_start[i]..row_start[i + 1] - 1, at positions
+    tensors, all on the regions' GPU: slot i's rows are row_start[i]..row_start[i + 1] - 1, at positions
     pos[i], pos[i] + 1, ... (row_start None: one row for each slot). pos -1
     marks a slot without rows. Calls enqueue on `stream` (a CUDA stream
     handle; None: the default stream) and do not wait."""
@@ -543,6 +545,7 @@ class Kv8Set:
                                    n_heads, C.byref(h)))
         self._h = h
         self.n, self.n_heads, self.spec = len(self.kvs), n_heads, self.kvs[0].spec
+        self.device = self.kvs[0].device
         self._nkv, self._hd = self.spec.n_kv_heads, self.spec.head_dim
         self._scale = self._hd ** -0.5
 
@@ -555,7 +558,7 @@ class Kv8Set:
 
     def append(self, layer, k, v, pos, row_start=None, stream=None):
         """Quantise rows of K and V [rows, n_kv_heads, head_dim] into `layer`."""
-        d = k.get_device()
+        d = self.device
         shape = (k.shape[0], self._nkv, self._hd)
         dt, st = _matrix(k, d, shape, "k")
         if _matrix(v, d, shape, "v", dt)[1] != st:
@@ -569,7 +572,7 @@ class Kv8Set:
         t = k if k is not None else v
         if t is None:
             raise ValueError("k and v are both None")
-        d = t.get_device()
+        d = self.device
         shape = (t.shape[0], self._nkv, self._hd)
         dt, st = _matrix(t, d, shape, "k" if k is not None else "v")
         if k is not None and v is not None and _matrix(v, d, shape, "v", dt)[1] != st:
@@ -581,7 +584,7 @@ class Kv8Set:
     def attend(self, layer, q, out, pos, row_start=None, scale=None, stream=None):
         """Causal attention of rows q [rows, n_heads, head_dim] over the cached
         positions up to each row's own, into out. scale None: head_dim ** -0.5."""
-        d = q.get_device()
+        d = self.device
         shape = (q.shape[0], self.n_heads, self._hd)
         dt, st = _matrix(q, d, shape, "q")
         ot = _matrix(out, d, shape, "out", dt)[1]
