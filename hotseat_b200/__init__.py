@@ -529,6 +529,11 @@ def _vector(t, device, n, name, dtype=-1):
     return t.data_ptr()
 
 
+def _same_strides(st, other, shape):
+    """Whether two matrices of one shape lie alike: rows or heads that are single have no stride."""
+    return st == other or all(n == 1 or a == b for a, b, n in zip(st, other, shape))
+
+
 class Kv8Set:
     """8-bit KV regions as the slots of batched calls (hs_kv8_set). Row
     matrices are device tensors [rows, heads, head_dim] (f32, f16 or bf16, any
@@ -561,7 +566,7 @@ class Kv8Set:
         d = self.device
         shape = (k.shape[0], self._nkv, self._hd)
         dt, st = _matrix(k, d, shape, "k")
-        if _matrix(v, d, shape, "v", dt)[1] != st:
+        if not _same_strides(_matrix(v, d, shape, "v", dt)[1], st, shape):
             raise ValueError("k and v must have the same strides")
         _check(_lib.hs_kv8_append(self._h, layer, shape[0], _vector(row_start, d, self.n + 1, "row_start"),
                                   _vector(pos, d, self.n, "pos"), k.data_ptr(), v.data_ptr(), dt, st[0], st[1],
@@ -575,7 +580,7 @@ class Kv8Set:
         d = self.device
         shape = (t.shape[0], self._nkv, self._hd)
         dt, st = _matrix(t, d, shape, "k" if k is not None else "v")
-        if k is not None and v is not None and _matrix(v, d, shape, "v", dt)[1] != st:
+        if k is not None and v is not None and not _same_strides(_matrix(v, d, shape, "v", dt)[1], st, shape):
             raise ValueError("k and v must have the same strides")
         _check(_lib.hs_kv8_read(self._h, layer, shape[0], _vector(row_start, d, self.n + 1, "row_start"),
                                 _vector(pos, d, self.n, "pos"), k.data_ptr() if k is not None else None,
