@@ -614,8 +614,8 @@ def logprobs(logits, ids=None, logp=None, entropy=None, rank=None, top_ids=None,
     for t, name, want in ((top_ids, "top_ids", -1), (top_logp, "top_logp", F32)):
         if t is None:
             continue
-        n = t.shape[1]
-        if t.get_device() != d or t.shape[0] != rows or (top and n != top) or _dtype(t) != want or not t.is_contiguous():
+        n = t.shape[-1] if t.dim() == 2 else -1
+        if t.get_device() != d or t.shape != (rows, n) or (top and n != top) or _dtype(t) != want or not t.is_contiguous():
             raise ValueError(f"{name} must be a consecutive [rows, top] tensor of {'int32' if want < 0 else 'float32'}")
         top = n
     _check(_lib.hs_logprobs(d, logits.data_ptr(), dt, st[0], rows, vocab, _vector(ids, d, rows, "ids"), top,

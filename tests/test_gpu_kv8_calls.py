@@ -1,6 +1,5 @@
 """What calls on 8-bit regions and logits refuse and take: places, strides and
 shapes of tensors."""
-import numpy as np
 import pytest
 
 import hotseat_b200 as hs
@@ -57,3 +56,13 @@ def test_strides_of_single_rows_and_heads_do_not_count(nkv, m):
     assert raw(kv)[0].shape[1] == 32
     with pytest.raises(ValueError):  # strides that do count
         s.append(0, torch.zeros(2, nkv, 128, device="cuda")[..., :64], torch.zeros(2, nkv, 64, device="cuda"), i32([0]), i32([0, 2]))
+
+
+def test_outputs_of_other_shapes_are_refused():
+    x, ids = torch.zeros(3, 50, device="cuda"), i32([1, 2, 3])
+    f, n = torch.zeros(3, device="cuda"), torch.zeros(3, 2, device="cuda")
+    for kw in (dict(top_logp=f), dict(top_logp=n[:2]), dict(top_logp=n[None]), dict(top_ids=n), dict(top_ids=ids),
+               dict(top_ids=torch.zeros(3, 4, dtype=torch.int32, device="cuda"), top_logp=n), dict(logp=f[:2], ids=ids),
+               dict(logp=n, ids=ids), dict(entropy=f.half()), dict(rank=f, ids=ids), dict(logp=f, ids=ids.long())):
+        with pytest.raises(ValueError):
+            hs.logprobs(x, **kw)
