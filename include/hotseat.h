@@ -227,7 +227,15 @@ uint64_t hs_runs_to_byte_runs(const uint64_t* words, uint64_t n_pages, uint64_t 
  * integer nearest to x / s, ties to even. A value is then within s / 2 of
  * what was stored, and within s where its block's scale grew after it. With
  * block 1 a row's bytes never change and do not depend on how a prompt was
- * cut into calls. */
+ * cut into calls.
+ *
+ * Going back: rows may be appended again from any position on, and the rows
+ * before it keep their values, as above. With block > 1 an append is the end of
+ * its last block: what that block holds behind the new rows has no meaning until
+ * it is appended too (an f32 region, and block 1, keep rows behind). The scale of
+ * the block that holds the position stays as large as the rows taken back had made
+ * it, NaN included, so its bytes are those of a sequence that never had these
+ * rows only where the append begins the block. */
 #define HS_F32 0u
 #define HS_F16 1u
 #define HS_BF16 2u

@@ -1,5 +1,6 @@
 """What calls on 8-bit regions and logits refuse and take: places, strides and
 shapes of tensors."""
+import numpy as np
 import pytest
 
 import hotseat_b200 as hs
@@ -66,3 +67,54 @@ def test_outputs_of_other_shapes_are_refused():
                dict(logp=n, ids=ids), dict(entropy=f.half()), dict(rank=f, ids=ids), dict(logp=f, ids=ids.long())):
         with pytest.raises(ValueError):
             hs.logprobs(x, **kw)
+
+
+@pytest.mark.parametrize("block, layout", [(1, 0), (16, 1), (64, 0)])
+def test_going_back(block, layout):
+    """Rows taken back and appended anew, in the middle of a block and at its beginning."""
+    rng = np.random.default_rng(block)
+    spec = hs.KvSpec(1, 2, 64, 200, layout)
+    kv, ref, fresh = hs.Kv.alloc8(spec, block=block), Cache(2, 64, 200, block), Cache(2, 64, 200, block)
+    s = hs.Kv8Set([kv])
+    x = (rng.standard_normal((200, 2, 64)) * np.exp(rng.uniform(-1, 1, (200, 1, 1)))).astype(np.float32)
+    steps = np.zeros((200, 2), np.float32)  # the largest scale that each row has stood under
+
+    def add(pos, rows):
+        t = torch.from_numpy(rows).cuda()
+        s.append(0, t, t, i32([pos]), i32([0, len(rows)]))
+        ref.append(pos, rows, rows)
+        now = ref.scales[0][np.arange(200) // block]
+        steps[:] = np.maximum(steps, now)
+
+    def values(n):
+        k = torch.empty(n, 2, 64, device="cuda")
+        s.read(0, k, None, i32([0]), i32([0, n]))
+        return k.cpu().numpy()
+
+    add(0, x[:150])
+    held = values(150)
+    big = 8 * x[:40]
+    add(100, big)  # in a block for 16 and 64; the rows before it stay within a step of its scale
+    got = values(140)
+    assert np.array_equal(got, ref.values(0, 0, 140))
+    assert np.array_equal(got[:100 // block * block], held[:100 // block * block])
+    assert np.all(np.abs(got[:100].astype(np.float64) - x[:100]) <= steps[:100, :, None] * (1 + 2 ** -20))
+    assert np.all(np.abs(got[100:].astype(np.float64) - big) <= steps[100:140, :, None] * (1 + 2 ** -20))
+    if block == 1:
+        assert np.array_equal(values(150)[140:], held[140:])  # rows behind stay
+    # taken back to the beginning of a block: a fresh sequence's bytes
+    back = 64
+    add(back, x[back:150])
+    fresh.append(0, x[:back], x[:back])
+    fresh.append(back, x[back:150], x[back:150])
+    codes, scales = raw(kv)
+    nb = -(-150 // block)
+    assert np.array_equal(scales[:, :nb], fresh.scales[:, :nb]) and np.array_equal(codes[:, :150], fresh.codes[:, :150])
+    # a row that is not finite, taken back: its block stays NaN where it held older rows
+    bad = np.full((1, 2, 64), np.nan, np.float32)
+    add(70, bad)
+    add(70, x[70:72])
+    got = values(72)
+    assert np.isnan(got[70]).all() == (block > 1) and np.array_equal(np.isnan(got[64:70]).all(), block > 1)
+    add(64, x[64:72])
+    assert not np.isnan(values(72)).any()
