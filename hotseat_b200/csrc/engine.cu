@@ -850,6 +850,22 @@ hs_kv_spec model_kv_spec(const hs_model* m, uint32_t layout) {
     return hs_kv_spec{m->cfg.n_layers, m->cfg.n_kv_heads, m->cfg.head_dim, m->cfg.max_ctx, layout};
 }
 
+// Bytes from `p` to the end of the allocation that holds it; ~0 where that
+// cannot be told.
+static uint64_t bytes_behind(const void* p) {
+    typedef CUresult (*RangeFn)(CUdeviceptr*, size_t*, CUdeviceptr);
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuMemGetAddressRange", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+        return ~0ull;
+    CUdeviceptr base = 0;
+    size_t size = 0;
+    const CUdeviceptr at = reinterpret_cast<CUdeviceptr>(p);
+    if (reinterpret_cast<RangeFn>(fn)(&base, &size, at) != CUDA_SUCCESS) return ~0ull;
+    return base + size - at;
+}
+
 int kv_create(int device, const hs_kv_spec& spec, uint32_t block8, uint32_t page_size, uint64_t fingerprint,
               const void* handle, hs_kv** out) {
     if (spec.layout > 1) return fail(HS_E_ARG, "unknown KV layout");
@@ -881,6 +897,8 @@ int kv_create(int device, const hs_kv_spec& spec, uint32_t block8, uint32_t page
         HS_CUDA_TRY(cudaIpcOpenMemHandle(&p, h, cudaIpcMemLazyEnablePeerAccess));
         kv->base = static_cast<float*>(p);
         kv->ipc_view = true;
+        // a handle says nothing of its region; a larger format would reach past it
+        if (bytes_behind(p) < bytes) return fail(HS_E_ARG, "the exported region is smaller than this shape and format");
     }
     HS_CUDA_TRY(cudaStreamCreateWithFlags(&kv->st, cudaStreamNonBlocking));
     if (!handle) {

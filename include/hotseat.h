@@ -102,7 +102,9 @@ int hs_kv_info(const hs_kv* kv, hs_kv_spec* spec, uint64_t* bytes, uint32_t* pag
  * process opens it with hs_kv_open_ipc on its own model and GPU, which maps
  * the remote region for hs_kv_peer_copy / hs_kv_copy_runs / hs_migrate_* as
  * a destination (stores over NVLink). A view is never decoded into; the
- * owner must keep its region alive until the view is freed (hs_kv_free). No
+ * owner must keep its region alive until the view is freed (hs_kv_free).
+ * HS_E_ARG if what the handle maps is smaller than a region of the shape and
+ * format asked for (a handle of an 8-bit region opened as an f32 one). No
  * counterpart in the reference, whose hand-over crosses a TCP socket
  * (hs-wire lib.rs:338-396). */
 #define HS_IPC_HANDLE_BYTES 64
