@@ -118,3 +118,59 @@ def test_going_back(block, layout):
     assert np.isnan(got[70]).all() == (block > 1) and np.array_equal(np.isnan(got[64:70]).all(), block > 1)
     add(64, x[64:72])
     assert not np.isnan(values(72)).any()
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_the_last_position_behind_4_gib(block):
+    """A row of its own there, read into other values, and found at its own bytes only."""
+    n = 1 << 20
+    spec = hs.KvSpec(3, 8, 128, n, 1)
+    kv = hs.Kv.alloc8(spec, block=block)
+    assert kv.bytes > 2 ** 32
+    s = hs.Kv8Set([kv], n_heads=8)
+    rng = np.random.default_rng(block)
+    k, kf = rows_of(rng, 3, 8, 128, "f32")
+    ref = Cache(8, 128, block, block)
+    ref.append(block - 1, kf[2:], kf[2:])  # the region's last block, of which it is the last row
+    s.append(2, k[:2], k[:2], i32([0]), i32([0, 2]))
+    first = torch.full_like(k[:2], 5.0)
+    s.read(2, first, None, i32([0]), i32([0, 2]))
+    s.append(2, k[2:], k[2:], i32([n - 1]))
+    for which in range(2):
+        back = torch.full_like(k[:1], 5.0)
+        s.read(2, *((back, None) if which == 0 else (None, back)), i32([n - 1]))
+        assert torch.equal(back.cpu(), torch.from_numpy(ref.values(which, block - 1, block)))
+    again = torch.full_like(k[:2], 5.0)
+    s.read(2, again, None, i32([0]), i32([0, 2]))
+    assert torch.equal(first, again)
+    # the code row of K's last head at the plane's end, of V's one plane on
+    plane = n * 8 * 128
+    at = 2 * (kv.bytes // 3)
+    for which in range(2):
+        row = kv.read(at + which * plane + plane - 128, 128).view(np.int8)
+        assert np.array_equal(row, ref.codes[which, block - 1, 7]) and row.any()
+    s.check()
+
+
+@pytest.mark.parametrize("block", [1, 16])
+def test_the_rounds_of_a_hand_over(tiny_gguf, block):
+    """What each round sends: the rows since the one before, from the start of the block that they continue."""
+    m = hs.Model.load(tiny_gguf, max_ctx=256, numeric=hs.NUMERIC_TC)
+    src, dst, b = m.kv8(block=block, page_size=256), m.kv8(block=block, page_size=256), hs.Batch(m, 64)
+    b.prefill(src, np.arange(100) % m.cfg.vocab)
+    g = hs.Migration(src, dst, 100, 101, target_bytes=0)
+    for p in range(100, 110):
+        b.forward([src], [p], [p])
+    assert g.round(110, 111) is True  # smaller than the whole, above the target of 0
+    assert g.round(110, 111) is False  # nothing was written since
+    for p in range(110, 113):
+        b.forward([src], [p], [p])
+    rep = g.finish(113, 114)
+    assert [r["index"] for r in rep["rounds"]] == [0, 1] and rep["converged"] == 1
+    assert rep["stop_reason"] == "nothing left to send"
+    sent = lambda a, z: sum(n for _, n in hs.live_ranges_between8(m.kv_spec(), block, a, z))  # noqa: E731
+    assert rep["rounds"][0]["bytes"] == sent(0, 101)
+    # pages that hold the ten rows, clipped to the live ranges from their block's start on
+    assert 10 * 2 * 2 * m.cfg.n_layers * 64 <= rep["rounds"][1]["bytes"] <= sent(100, 111)
+    assert 0 < rep["final_bytes"] <= sent(110, 113) and rep["live_bytes"] == sent(0, 113)
+    assert dst.hash(113) == src.hash(113)
