@@ -2131,17 +2131,15 @@ int batch_attend_kv8(hs_batch* b, const SplitAttnArgs& sa, uint32_t n, bool pref
     a.kv.base = b->kv_tab;
     a.kv.dirty = b->dirty_tab;
     a.kv.tracking = b->track_tab;
-    a.kv.n_slots = prefill ? 1 : n;
     a.kv.page_shift = b->page_shift;
     a.rows.n_rows = n;
-    a.rows.n_slots = a.kv.n_slots;
+    a.rows.n_slots = prefill ? 1 : n;
     a.rows.row_start = prefill ? b->start8 : nullptr;
     a.rows.pos = b->pos8;
     a.rows.err = b->err;
     a.q = Kv8Mat{b->q8, (uint64_t)c.n_heads * hd, hd, HS_F32};
     a.out = Kv8Mat{b->o8, (uint64_t)c.n_heads * hd, hd, HS_F32};
     a.q_vec = a.out_vec = true;
-    a.nh = c.n_heads;
     a.scale = 1.0f / std::sqrt((float)hd);
     kv8_use_plan(&a, b->plan8);
     a.part = b->part8;

@@ -15,7 +15,6 @@
 
 namespace hs {
 
-constexpr uint32_t kKv8MaxBlock = 128;
 constexpr uint32_t kPosNone = 0xffffffffu;  // HS_POS_NONE
 
 struct Kv8Geo {
@@ -42,7 +41,7 @@ struct Kv8View {
     uint64_t layer_off = 0, plane = 0, splane = 0;
     uint64_t pos_stride = 0, head_stride = 0;    // codes, bytes
     uint64_t sblk_stride = 0, shead_stride = 0;  // scales, elements
-    uint32_t n_slots = 0, nkv = 0, max_ctx = 0, block_shift = 0, page_shift = 0;
+    uint32_t nkv = 0, max_ctx = 0, block_shift = 0, page_shift = 0;
 
     __device__ uint64_t code_off(uint32_t v, uint32_t head, uint32_t pos) const {
         return layer_off + (v ? plane : 0) + (uint64_t)pos * pos_stride + (uint64_t)head * head_stride;
@@ -132,7 +131,7 @@ struct Kv8AttendArgs {
     Kv8View kv;
     Kv8Rows rows;
     Kv8Mat q, out;
-    uint32_t nh = 0, group = 0, chunks = 0;  // query heads, per KV head, and CTAs of kv8_single_cols for these
+    uint32_t group = 0, chunks = 0;  // query heads of a KV head, and CTAs of kv8_single_cols for these
     float scale = 1.0f;
     uint32_t slot_clusters = 0;  // split chunks: clusters set aside for each slot; 0: for each tile that the rows can need
     bool q_vec = false, out_vec = false;  // four elements of a row at once: base and strides allow it
@@ -182,37 +181,5 @@ struct SplitAttnArgs;
 cudaError_t launch_kv8_qkv_rows(uint32_t hd, const SplitAttnArgs& a, uint32_t slots, float* q, float* k, float* v,
                                 uint32_t* pos, uint32_t* row_start, cudaStream_t st);
 cudaError_t launch_kv8_to_pairs(const float* x, uint64_t n, uint16_t* hi, uint16_t* lo, cudaStream_t st);
-
-#ifdef __CUDACC__
-// Row `r` of the batch: its slot and position. False for a row that is not
-// there (behind the last sequence, no position, or past max_ctx: flagged).
-__device__ __forceinline__ uint32_t kv8_slot_of(const Kv8Rows& rows, uint32_t r) {
-    if (!rows.row_start) return r;
-    uint32_t lo = 0, hi = rows.n_slots;  // the last slot whose first row is <= r and that is not empty
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (__ldg(rows.row_start + mid + 1) <= r)
-            lo = mid + 1;
-        else
-            hi = mid;
-    }
-    return lo;  // n_slots: behind the last sequence
-}
-__device__ __forceinline__ bool kv8_place(const Kv8Rows& rows, uint32_t max_ctx, uint32_t r, uint32_t* slot,
-                                          uint32_t* pos) {
-    const uint32_t s = kv8_slot_of(rows, r);
-    if (s >= rows.n_slots) return false;
-    const uint32_t first = rows.row_start ? __ldg(rows.row_start + s) : r, p0 = __ldg(rows.pos + s);
-    if (p0 == kPosNone || first > r) return false;
-    const uint64_t p = (uint64_t)p0 + (r - first);
-    if (p >= max_ctx) {
-        atomicOr(rows.err, 4u /* ERR_POS */);
-        return false;
-    }
-    *slot = s;
-    *pos = (uint32_t)p;
-    return true;
-}
-#endif
 
 }  // namespace hs

@@ -90,7 +90,6 @@ Kv8View view_of(const hs_kv8_set* s, uint32_t layer) {
     v.base = reinterpret_cast<float* const*>(s->tab);
     v.dirty = reinterpret_cast<uint64_t* const*>(s->tab + s->n);
     v.tracking = reinterpret_cast<const uint32_t* const*>(s->tab + 2 * s->n);
-    v.n_slots = s->n;
     v.page_shift = s->page_shift;
     return v;
 }
@@ -275,7 +274,6 @@ int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t
     a.rows = rows_of(s, n_rows, row_start, pos);
     a.q = Kv8Mat{q, q_row_stride, q_head_stride, dtype};
     a.out = Kv8Mat{out, out_row_stride, out_head_stride, dtype};
-    a.nh = s->nh;
     kv8_use_plan(&a, s->plan);
     a.scale = scale;
     a.q_vec = fours(a.q);
