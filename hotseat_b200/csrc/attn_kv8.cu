@@ -142,6 +142,9 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // A single row per slot. One CTA takes a split of the positions of one (slot,
 // KV head), its warps blocks of BP positions in turn. A warp computes
@@ -528,9 +531,9 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
             if (d == 0 || i == i0) rec[stats + col] = mm, rec[stats + NC + col] = ll;
         }
     }
-    // no CTA leaves while others read its record
+    // no CTA leaves while others read its record: their reads lie before the barrier
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+    cluster_sync();
     if (n_cl == 1) return;
 
     // more clusters: the last one to finish this share joins their records in order
@@ -650,10 +653,6 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 template <uint32_t N = 128>
 __device__ __forceinline__ void bar_sync(uint32_t id) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
-}
-
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <int HD, int DT, bool SPLIT>
