@@ -162,12 +162,15 @@ __device__ __forceinline__ void cluster_sync() {
 // distributed shared memory, each CTA a share of the outputs; where a row has
 // more, each share's last cluster joins the clusters' records in order.
 //
-// Bound by the instructions between a block's arrival and the next (about 515
-// a warp for 4 KB of codes, in a chain of ~1,700 clocks; four warps an SM
-// quarter hide part of it) and, below ~2,000 positions, by the CTA's start and
-// join. 64 rows of 14/2 heads of 64, f32, up to 2,048 positions: 15 us, 3.6 at
-// the memory's rate; 8,192 positions each: 46 us (2.9 TB/s of codes); one row:
-// 5.9 us at 2,048 positions, 16 at 32,768 (12/2 heads of 128).
+// Bound by issue and by chains of dependent instructions: about 515 a warp for
+// a block's 4 KB of codes, four fifths of all at 64 x 8,192 positions, where the
+// schedulers issue in 48 % of their clocks and the first stalls are fixed
+// latencies and the CTA's barriers; below ~2,000 positions by the CTA's start and
+// joins. The grid has every split that the region's max_ctx allows, and CTAs
+// without one leave at once. 64 rows of 14/2 heads of 64, f32, up to 2,048
+// positions: 17.5 us, 3.6 at the memory's rate; 8,192 positions each: 46 us
+// (3.1 TB/s); one row: 6.2 us at 2,048 positions, 15.5 at 32,768 (12/2 heads of
+// 128, f16).
 template <int HD, int DT, int NT>
 struct DecGeom {
     static constexpr uint32_t BP = HD == 64 ? 32 : 16;  // positions of a block: 4 KB of codes either way
@@ -575,9 +578,10 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 //                   from, the tile's outputs from TMEM into f32 registers;
 //                   the first thread issues the tile's MMAs
 //   warps 8-15      codes from the cache to f16 tiles in shared memory, 16
-//                   positions a warp: K as it lies, V transposed. A warp loads
-//                   a tile's codes into registers as it writes the one
-//                   before, and waits for no other warp.
+//                   positions a warp (f32 rows: warps 8-11, 32 positions): K as
+//                   it lies, V transposed. A warp loads a tile's codes into
+//                   registers as it writes the one before, and waits for no
+//                   other warp.
 //
 //   S = Q K^T    A = Q (shared), B = K (shared), 128 x 128
 //   O' = W V     A = W (TMEM),   B = V^T (shared), 128 x head_dim
@@ -590,19 +594,19 @@ __global__ void __launch_bounds__(DecGeom<HD, DT, NT>::THREADS, NT == 1 ? 4 : 2)
 // leave outputs, maxima and sums in shared memory, and each joins a share of
 // the rows.
 //
-// Bound by the row warps' softmax (exponentials, pairs, TMEM round trips; about
-// 3,100 clocks for 128 x 128 scores a warp in bf16, 5,800 with f32's pairs)
-// and by the CTA's start (12,000 clocks: q, the scales' maxima, the first
-// codes), not by the products. 12/2 heads of 128, 2,048 rows a slot: 8 slots in
-// bf16 205 us (502 TFLOP/s of the 1,630 measured); 4 in f32 183 us (282, each
-// product of pairs counted once).
+// Bound by the row warps' softmax (exponentials, pairs, TMEM round trips), not by
+// the products: a step of 256 x 128 scores takes 4.1 us at head_dim 64 and 4.9 at
+// 128 in 16 bits, 4.3 and 6.2 in f32. A CTA's start, masked step and end take 16
+// to 21 us (TMEM, q, the first codes; the outputs through shared memory).
+// 12/2 heads of 128, 2,048 rows a slot: 8 slots in bf16 281 us (367 TFLOP/s of
+// the 1,630 measured, each product of pairs counted once); 4 in f32 184 us (280).
 template <int HD, int DT>
 struct ChunkGeom {
     static constexpr bool QPAIR = DT == HS_F32;
     static constexpr uint32_t KT = 128, ROWS = 256;
     // f32 rows take each tile's O' out of TMEM and sum it in registers, rounded
     // to nearest: left to grow there, 2,048 positions were 1.7e-6 off (the
-    // tensor cores' sums truncate), so 5e-7. Their row warps get 192 registers a
+    // tensor cores' sums truncate), so 7.5e-7. Their row warps get 192 registers a
     // thread, and four code warps, of 120, do with the rest.
     static constexpr bool OREG = DT == HS_F32;
     static constexpr uint32_t CW = OREG ? 4 : 8, THREADS = 256 + 32 * CW, SUB = 8 / CW;

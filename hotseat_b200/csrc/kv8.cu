@@ -230,8 +230,9 @@ struct Walk {
 
 // Append, a scale for every position: a warp takes `per` rows in turn, HD / 8
 // lanes a head. The row's slot is searched once a row, the same for all lanes.
-// Bound by the latency of a row's chain (slot, loads, maximum, codes): 64 rows
-// of 2 heads of 64, f32: 2.8 us, of which a launch is 2.
+// Bound by the latency of a row's chain (slot, loads, maximum, codes, the fence
+// behind the stores): 64 rows of 2 heads of 64, f32: 3.4 us, of which a launch is
+// 2 and the fence 0.6.
 template <int HD, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
                                                           const Kv8Mat v, uint32_t per) {
@@ -290,8 +291,9 @@ __global__ void __launch_bounds__(kThreads) k_append_rows(const Kv8View kv, cons
 // and the codes, RL rows a lane; the unit's older rows are rescaled where the
 // scale doubles. Units of slot i start at unit row_start[i] / B + 2 i, which
 // leaves room for every block that its rows can touch. Bound by the latency of
-// loading, reducing and storing in turn: 16 x 2,048 rows of 2 heads of 128,
-// bf16, blocks of 32: 25 us (2.0 TB/s moved).
+// loading, reducing, storing and waiting for the stores in turn, a unit a warp
+// with nothing of the next on its way: 16 x 2,048 rows of 2 heads of 128, bf16,
+// blocks of 32: 30 us (1.7 TB/s moved), five of them the stores' end.
 template <int HD, int DT, bool VEC, int B>
 __global__ void __launch_bounds__(kThreads) k_append_blocks(const Kv8View kv, const Kv8Rows rows, const Kv8Mat k,
                                                             const Kv8Mat v) {

@@ -95,7 +95,7 @@ cudaError_t launch_kv8_read(uint32_t hd, const Kv8View& kv, const Kv8Rows& rows,
 // region's shape alone, so that its bits do not depend on the batch: in
 // eight (a cluster), but splits of at least 32 KB and at most 128 KB of codes
 // and no more than kv8_max_splits. Short splits finish a lone row sooner (2,048
-// positions, 14/2 heads of 64: 5.9 us in eight, 7.6 in four), long ones keep a
+// positions, 14/2 heads of 64: 6.2 us in eight, 7.6 in four), long ones keep a
 // large batch's CTAs from spending their time on starting and joining (64
 // sequences of 8,192: 46 us with 128 KB, 58 with 64 KB).
 constexpr uint32_t kv8_max_splits(uint32_t nkv) {
@@ -116,9 +116,11 @@ constexpr uint32_t kv8_single_cols(uint32_t group) { return group <= 8 ? 8 : 16;
 // (row, head) pairs, by the slot's own rows (`tiles` of them, from position
 // pos0 on) and the region's shape alone: where a slot's tiles are few, and for
 // 512 positions a CTA at least. 16 rows a slot, 12/2 heads of 128, bf16, over
-// 5,000 positions: 25 us shared, 110 by one CTA for each KV head; 16 such slots
-// 72 and 112; 64 slots, which fill the GPU by themselves and pay for the CTAs'
-// starts and joins, 234 and 117. One slot over 32,768 positions: 93 and 647.
+// 5,000 positions: 33 us shared, 169 by one CTA for each KV head; 16 such slots
+// 93 and 166; 64 slots, which fill the GPU by themselves and pay for the CTAs'
+// starts and joins, 290 and 171 (at 9,000: 428 and 294). One slot over 9,000: 48
+// and 293, over 32,768: 139 and 1,035. The rule is for the slot alone; a large
+// batch of such rows pays for it.
 constexpr uint32_t kKv8ChunkSplits = 8, kKv8ChunkClusters = 8;  // CTAs of a cluster, clusters of a slot
 __host__ __device__ constexpr bool kv8_chunk_shared(uint64_t tiles, uint32_t pos0, uint32_t nkv) {
     return tiles * nkv <= kKv8ChunkClusters && pos0 >= 512 * kKv8ChunkSplits;

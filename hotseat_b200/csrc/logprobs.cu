@@ -24,7 +24,10 @@
 // lists the same way.
 //
 // A share that is longer than a CTA holds (20,480 logits) goes through the
-// registers in strips, their results joined in turn.
+// registers in strips, their results joined in turn. A strip costs the same
+// whatever is in it, so a row costs its strips: 2,048 rows in bf16, all outputs,
+// top 5, take 400 us at 151,936, 128,256, 102,400 and 32,000 tokens, 453 at
+// 50,257, whose rows are not aligned, and 733 at 256,000, where every share has two.
 //
 // Bound by the instructions of a logit (about a dozen) and the barriers of a
 // strip: 2,048 rows of 151,936 in bf16: entropy alone 294 us (2.1 TB/s), with

@@ -291,9 +291,12 @@ int hs_kv8_read(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* 
 /* Causal attention: the row at position p of slot i attends positions 0..p of
  * region i (so append its K and V first) with its n_heads query heads, query
  * head h on KV head h / (n_heads / n_kv_heads): softmax(scale * q.k) . v.
- * Statistics and sums are f32; a row's bits do not depend on the other slots
- * of the batch, but on the form (row_start or none) and, with row_start, on
- * which rows of its own slot the call holds. `out` must not overlap `q`. */
+ * Statistics and sums are f32, codes exact, q and weights of 22 bits at least
+ * under a power of two, for every type; the result is rounded once. Positions
+ * behind a row's own do not change it, whatever they hold. Scores whose sum of
+ * products passes f32's range give NaN. A row's bits do not depend on the other
+ * slots of the batch, but on the form (row_start or none) and, with row_start,
+ * on which rows of its own slot the call holds. `out` must not overlap `q`. */
 int hs_kv8_attend(hs_kv8_set* s, uint32_t layer, uint32_t n_rows, const uint32_t* row_start, const uint32_t* pos,
                   const void* q, uint64_t q_row_stride, uint64_t q_head_stride, void* out, uint64_t out_row_stride,
                   uint64_t out_head_stride, uint32_t dtype, float scale, void* stream);
